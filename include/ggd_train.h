@@ -132,6 +132,64 @@ int ggd_tr_pixel_shuffle(int N, int H, int W, int C, int r, const float* src, fl
 /* head flatten (ResNetSE34V2.py:161-165): NHWC [N][H][W][C] -> rows (n, w) x features (c H + h). */
 int ggd_tr_head_flatten(int N, int H, int W, int C, const float* src, float* dst, int backward, void* stream);
 
+/* ---- operators of a decoder block beyond the reference's (…_amd/blocks.py) ---- */
+enum { GGD_TR_F32 = 0, GGD_TR_BF16 = 1 };             /* dtype of the row tensors; weights and statistics are f32 */
+enum { GGD_TR_LAYERNORM = 0, GGD_TR_RMSNORM = 1 };    /* kind */
+
+/* The norms around a block with its gate and residual scale, over contiguous rows of d <= 8192:
+ *   h_out = scale h + gate * post(y),  u = pre(h_out before its rounding)
+ * post / pre: LayerNorm (eps) or RMS norm with weight *_g and bias *_b (nullable; post_g null: no post
+ * norm).  gate (nullable): row r takes gate row r / gate_rows, and gate_rows divides rows.  stats
+ * (nullable where no backward pass follows): [4][rows].  A shape beyond the limits is -2.
+ * Backward: from the gradients dh_out and du, dh, dy, dgate (with a gate) and the weights' -- those
+ * of the weights given, all of them overwritten.  ws: ggd_tr_resnorm_ws(...) bytes, 16-byte aligned,
+ * used by this call alone until it has run.  Every sum has a fixed order. */
+int ggd_tr_resnorm_fwd(int64_t rows, int d, int dtype, int kind, float scale, float eps, const void* h, const void* y,
+                       const void* gate, int64_t gate_rows, const float* post_g, const float* post_b, const float* pre_g,
+                       const float* pre_b, void* h_out, void* u, float* stats, void* stream);
+int ggd_tr_resnorm_bwd(int64_t rows, int d, int dtype, int kind, float scale, float eps, const void* h, const void* y,
+                       const void* gate, int64_t gate_rows, const float* post_g, const float* post_b, const float* pre_g,
+                       const float* pre_b, const float* stats, const void* dh_out, const void* du, void* dh, void* dy,
+                       void* dgate, float* d_post_g, float* d_post_b, float* d_pre_g, float* d_pre_b, void* ws,
+                       int64_t ws_bytes, void* stream);
+int64_t ggd_tr_resnorm_ws(int64_t rows, int d, int64_t gate_rows, int has_gate);
+
+/* Attention for any lengths, with masks, kv heads shared by query heads, and a learned relative position
+ * bias; heads of dk <= 128 elements, f32 or bf16 (sums and softmax in f32):
+ *   s_ij = scale q_i . k_j + table[bucket(j - i - offset)][head],  o_i = sum_j softmax_j(s_ij) v_j
+ * over the keys that mask allows; a row with none is zeros.  Query head h reads kv head h / (heads / kv_heads).
+ * Memory of masked keys and queries is not read: whatever it holds reaches nothing. */
+typedef struct ggd_tr_battn_args {
+  int32_t n, heads, kv_heads, lq, lk, dk;  /* lq, lk >= 1 */
+  int32_t dtype;                           /* GGD_TR_F32 / GGD_TR_BF16 */
+  float scale;                             /* > 0 */
+  /* rows of heads (kv_heads) dk contiguous elements; strides in elements, ld* between rows, b* between clips */
+  const void *q, *k, *v;
+  void* o;
+  int64_t ldq, bq, ldk, bk, ldv, bv, ldo, bo;
+  const uint8_t *mask, *q_mask;            /* nullable: [n][lk], [n][lq] bytes, nonzero = there; strides between clips */
+  int64_t bmask, bq_mask;
+  /* bias, nullable: table [n_buckets][heads]; buckets [2 distance + 1]: the bucket of each clamped distance
+   * -distance .. distance.  A table entry of -inf forbids its places. */
+  const float* table;
+  const int32_t* buckets;
+  int32_t n_buckets, distance;             /* <= 1024, <= 2047 */
+  int64_t offset;                          /* position of query row 0 less that of key 0 */
+  /* kept for the backward pass (both null where none follows): [n][heads][lq][2], and o in f32, [n][lq][heads dk]
+   * (f32: may be o itself where its rows are contiguous) */
+  float *stat, *o32;
+  /* backward: dout, dq like o32's rows, dk and dv [n][lk][kv_heads dk], contiguous; dtable (nullable) [n_buckets][heads] */
+  const void* dout;
+  void *dq, *dk_out, *dv;
+  float* dtable;
+  void* ws;                                /* ggd_tr_battn_ws bytes, 16-byte aligned, this call's alone until it has run */
+  int64_t ws_bytes;
+} ggd_tr_battn_args;
+int ggd_tr_battn_fwd(const ggd_tr_battn_args* args, void* stream);
+/* reads q, k, v, masks, table, stat, o32, dout; writes dq, dk_out, dv, dtable.  Every sum has a fixed order. */
+int ggd_tr_battn_bwd(const ggd_tr_battn_args* args, void* stream);
+int64_t ggd_tr_battn_ws(const ggd_tr_battn_args* args, int backward);
+
 #ifdef __cplusplus
 }
 #endif

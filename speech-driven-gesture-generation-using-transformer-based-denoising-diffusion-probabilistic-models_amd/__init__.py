@@ -9,6 +9,7 @@ the reference's create_model / Generator / JsonConfig surface.
 The decoder and the diffusion update run as hand-written gfx950 kernels in
 libggd.so (csrc/), reached through its C ABI (include/ggd.h) with ctypes.
 """
+from .blocks import RelativeBuckets, cross_attention, relative_attention, residual_norm
 from .config import JsonConfig, adapt_legacy, load_config
 from .diffusion import (GaussianDiffusion, GaussianSpacedDiffusion, InpaintDenoise, get_named_beta_schedule,
                         space_timesteps)
@@ -21,5 +22,5 @@ __all__ = [
     "JsonConfig", "adapt_legacy", "load_config", "GaussianDiffusion", "GaussianSpacedDiffusion",
     "InpaintDenoise", "get_named_beta_schedule", "space_timesteps", "Generator", "Speech2GestureModel",
     "create_diffusion", "create_model", "sync_all", "arch_from_config", "count_parameters", "init_state_dict",
-    "parameter_shapes",
+    "parameter_shapes", "RelativeBuckets", "cross_attention", "relative_attention", "residual_norm",
 ]

@@ -1,0 +1,314 @@
+// ggd_battn.h -- attention of the training path for any lengths (gfx950): masks, shared kv heads, a
+// learned relative position bias, f32 and bf16, forward and backward (include/ggd_train.h,
+// ggd_tr_battn_*).
+//
+//   s_ij = scale q_i . k_j + table[bucket(j - i - offset)][head],  p = softmax over the allowed j
+//   o_i  = sum_j p_ij v_j          (a row with no allowed key: o_i = 0, no gradient)
+//   delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dq = scale ds k,  dk = scale ds^T q,  dv = p^T do,  dtable[b][head] = sum of ds over the bucket
+//
+// Every kernel keeps one operand's rows in registers -- lane & 31 = the row -- and streams the other
+// side's rows through LDS in tiles.  A product "streamed x stationary" then has the streamed rows
+// as the MFMA's M and the stationary row as the lane, so that a stationary row's scores lie in the
+// registers of two lanes (l and l ^ 32), the softmax needs one exchange between them, and the
+// probabilities are at once the B operand of the next product: its k slots may hold the streamed rows
+// in any order, as long as the A operand uses the same one (bt_acc).  No score goes through LDS.
+//   forward, dq:  stationary = queries (q, do), streamed = keys (k, v)
+//   dk, dv:       stationary = keys (k, v),     streamed = queries (q, do)
+// dq and dk / dv are two kernels that both form the scores (7 products instead of 5): the sums over
+// the streamed side then stay in registers, with neither atomics nor an order that varies.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "ggd_common.h"
+
+#include "../../include/ggd_train.h"
+
+namespace ggd {
+namespace battn {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+
+constexpr int BT_MAX_DK = 128, BT_MAX_DISTANCE = 2047, BT_MAX_BUCKETS = 1024;
+constexpr float BT_LOG2E = 1.4426950408889634f;
+
+struct BtArgs : ggd_tr_battn_args {
+  int group;       // query heads of a kv head
+  int off;         // offset, clamped (past the table's distance on either side all is one bucket)
+  int splits;      // parts of the streamed axis (few, dq, dkv)
+  int vec;         // rows are 16-byte aligned and dk a multiple of 16 bytes
+  int vec_o;       // the written rows take 4-element stores
+  float c;         // scale log2(e): scores are held in log2 units
+  float* part;     // partial results of the splits
+  float* delta;    // [n][heads][lq]
+  float* dtab;     // partial table gradients [blocks][n_buckets]
+  float* rest;     // bf16 with a table gradient: [splits][2][n][heads][lq], what the dq kernel leaves to bt_table_rest_kernel
+};
+
+// ---------------------------------------------------------------------------------------------
+// LDS images: rows of DK elements in 16-byte units, unit u of row r at u ^ swz(r).  64 banks of 4
+// bytes take 16 units at a time.  A row-wise read (lane = row, one unit each) needs 16 consecutive
+// rows in different units mod 16; bf16's transposing read (4 rows x 64 bytes) needs the units
+// 4 b .. 4 b + 3 of rows 4 a .. 4 a + 3 in different ones; swz is a bijection of the row bits that does both.
+// ---------------------------------------------------------------------------------------------
+template <typename T, int DK>
+struct Img {
+  static constexpr int EPU = 16 / sizeof(T), UPR = DK / EPU;
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (sizeof(T) == 2) {
+      if constexpr (UPR == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+      else if constexpr (UPR == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+      else return (r >> 2) & 3;
+    } else {
+      if constexpr (UPR >= 16) return r & 15;
+      else return (r >> 1) & 7;
+    }
+  }
+  static __device__ __forceinline__ int unit(int r, int u) { return r * UPR + (u ^ swz(r)); }
+};
+
+// rows of a streamed tile: one word of validity bits, one 64-lane load of the mask
+template <typename T, int DK>
+constexpr int tile_rows() { return sizeof(T) == 4 && DK == 128 ? 32 : 64; }
+
+__device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
+
+// byte of row r (r + lane) of a mask, or whether the row exists
+__device__ __forceinline__ int mask_byte(const uint8_t* mask, int row0, int rows, int count) {
+  const int l = lane_id(), r = row0 + l;
+  if (l >= rows || r >= count) return 0;
+  return mask ? mask[r] : 1;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 load_unit(const T* __restrict__ row, int u, int dk, bool vec) {
+  constexpr int EPU = 16 / sizeof(T);
+  const int c = u * EPU;
+  if (vec) return c < dk ? *(const uint4*)(row + c) : make_uint4(0, 0, 0, 0);
+  union { T e[EPU]; uint4 v; } x;
+  x.v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < EPU; ++i)
+    if (c + i < dk) x.e[i] = row[c + i];
+  return x.v;
+}
+
+// One tile of rows on its way from memory to an LDS image: THREADS threads hold N units each.  Rows
+// whose bit is clear are not read; they are zeros in the image, whatever memory holds there.
+template <typename T, int DK, int ROWS, int THREADS>
+struct Stage {
+  static constexpr int UPR = Img<T, DK>::UPR, N = ROWS * UPR / THREADS;
+  static_assert(ROWS * UPR % THREADS == 0, "whole units a thread");
+  uint4 x[N];
+  __device__ __forceinline__ void load(const T* __restrict__ base, int64_t ld, uint64_t bits, int dk, bool vec, int t) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = t + i * THREADS, r = e / UPR, u = e % UPR;
+      x[i] = (bits >> r) & 1 ? load_unit(base + r * ld, u, dk, vec) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void store(uint4* img, int t) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = t + i * THREADS, r = e / UPR, u = e % UPR;
+      img[Img<T, DK>::unit(r, u)] = x[i];
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// products.  acc: lane & 31 = the stationary row n, register 4 g + j of half h = lane >> 5 holds m = 8 g + 4 h + j
+// ---------------------------------------------------------------------------------------------
+// a stationary row's elements as B operands: unit 2 s + h of the row (bf16: 8 elements, one 32x32x16
+// product; f32: 4 elements, one 32x32x2 product each)
+template <typename T, int DK>
+struct Frag {
+  static constexpr int N = Img<T, DK>::UPR / 2;
+  uint4 x[N];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int dk, bool vec, bool there) {
+    const int h = lane_id() >> 5;
+#pragma unroll
+    for (int s = 0; s < N; ++s) x[s] = there ? load_unit(row, 2 * s + h, dk, vec) : make_uint4(0, 0, 0, 0);
+  }
+};
+
+// acc += rows r0 .. r0 + 31 of the image times the stationary rows (contraction over the elements)
+template <typename T, int DK>
+__device__ __forceinline__ void mma_rows(f32x16& acc, const uint4* img, int r0, const Frag<T, DK>& b) {
+  const int l = lane_id(), r = r0 + (l & 31), h = l >> 5;
+#pragma unroll
+  for (int s = 0; s < Frag<T, DK>::N; ++s) {
+    const uint4 a = img[Img<T, DK>::unit(r, 2 * s + h)];
+    if constexpr (sizeof(T) == 2) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b.x[s]), acc, 0, 0, 0);
+    } else {
+      const f32x4 af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b.x[s]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(af[j], bf[j], acc, 0, 0, 0);
+    }
+  }
+}
+
+// acc[mb] += (columns 32 mb .. + 31 of image rows r0 .. r0 + 31)^T times p, p as an acc of those rows.
+// bf16: p is rounded to bf16 here (half a step, 2^-9 of each weight, on sums that stay in f32); k slot 8 h + i
+// of step s is row 16 s + 8 (i / 4) + 4 h + i % 4 -- the rows the half's registers hold -- read by two
+// transposing loads.  f32: k slot h of step (g, j) is row 8 g + 4 h + j.
+// sum (SUM): + this half's weights as they go into the product, after their rounding
+template <typename T, int DK, bool SUM = false>
+__device__ __forceinline__ void mma_cols(f32x16 (&acc)[DK / 32], const uint4* img, int r0, const f32x16& p, float* sum = nullptr) {
+  const int l = lane_id(), h = l >> 5;
+  if constexpr (sizeof(T) == 2) {
+    const int i = l & 15, q = i >> 2;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint4 pb = make_uint4(pk_bf16(p[8 * s], p[8 * s + 1]), pk_bf16(p[8 * s + 2], p[8 * s + 3]),
+                                  pk_bf16(p[8 * s + 4], p[8 * s + 5]), pk_bf16(p[8 * s + 6], p[8 * s + 7]));
+      if constexpr (SUM) {
+        typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+        const bf16x2 ones = __builtin_bit_cast(bf16x2, 0x3F803F80u);
+        const uint32_t w[4] = {pb.x, pb.y, pb.z, pb.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[e]), ones, *sum, false);
+      }
+      const int ra = r0 + 16 * s + 4 * h + q, rb = ra + 8;
+#pragma unroll
+      for (int mb = 0; mb < DK / 32; ++mb) {
+        const int u = 4 * mb + 2 * ((l >> 4) & 1) + ((i & 3) >> 1);
+        typedef __attribute__((address_space(3))) bf16x4* lds4;
+        const bf16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)((uint2*)(img + Img<T, DK>::unit(ra, u)) + (i & 1)));
+        const bf16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)((uint2*)(img + Img<T, DK>::unit(rb, u)) + (i & 1)));
+        const bf16x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, pb), acc[mb], 0, 0, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = r0 + 8 * g + 4 * h + j;
+#pragma unroll
+        for (int mb = 0; mb < DK / 32; ++mb) {
+          const int u = 8 * mb + ((l & 31) >> 2);
+          const float a = ((const float*)(img + Img<T, DK>::unit(r, u)))[l & 3];
+          acc[mb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[4 * g + j], acc[mb], 0, 0, 0);
+        }
+      }
+  }
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// the other half's value (lane ^ 32) combined with this lane's, the same in both
+__device__ __forceinline__ float both_max(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float both_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// register 4 g + j of this half: row 8 g + 4 h + j of its block of 32
+__device__ __forceinline__ int reg_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// whether register r's row has its bit set; w: the block's 32 bits
+__device__ __forceinline__ bool row_bit(uint32_t w4, int r) { return (w4 >> (8 * (r >> 2) + (r & 3))) & 1; }   // w4 = w >> 4 h
+
+// a lane's row as it is written: 4 consecutive elements of columns 32 mb + 8 g + 4 h
+template <typename T, int DK>
+__device__ __forceinline__ void store_row(T* __restrict__ row, const f32x16 (&acc)[DK / 32], float f, int dk, bool vec) {
+  const int h = lane_id() >> 5;
+#pragma unroll
+  for (int mb = 0; mb < DK / 32; ++mb)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * mb + 8 * g + 4 * h;
+      const float v0 = acc[mb][4 * g] * f, v1 = acc[mb][4 * g + 1] * f, v2 = acc[mb][4 * g + 2] * f, v3 = acc[mb][4 * g + 3] * f;
+      if (vec) {
+        if (c >= dk) continue;
+        if constexpr (sizeof(T) == 4) *(f32x4*)(row + c) = f32x4{v0, v1, v2, v3};
+        else *(uint2*)(row + c) = make_uint2(pk_bf16(v0, v1), pk_bf16(v2, v3));
+      } else {
+        if (c < dk) row[c] = from_f32<T>(v0);
+        if (c + 1 < dk) row[c + 1] = from_f32<T>(v1);
+        if (c + 2 < dk) row[c + 2] = from_f32<T>(v2);
+        if (c + 3 < dk) row[c + 3] = from_f32<T>(v3);
+      }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// the bias: line[d + D] for d = clamp(j - i - offset, -D, D), in log2 units.  An entry of -inf forbids
+// its places; a finite one past the largest log2 unit counts as that, so that rows of the type's lowest
+// value stay a softmax among equals.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ float bias_entry(float x) {
+  constexpr float most = 2.358e38f;   // largest finite / log2(e)
+  return x == -INFINITY ? x : fminf(fmaxf(x, -most), most) * BT_LOG2E + (x != x ? x : 0.f);
+}
+__device__ __forceinline__ int bucket_of(const BtArgs& a, int d) {   // d in 0 .. 2 D
+  return min(max(a.buckets[d], 0), a.n_buckets - 1);
+}
+__device__ __forceinline__ void bias_line(float* line, const BtArgs& a, int head) {
+  for (int d = threadIdx.x; d <= 2 * a.distance; d += blockDim.x)
+    line[d] = bias_entry(a.table[(int64_t)bucket_of(a, d) * a.heads + head]);
+}
+
+// s (raw products) -> log2 units with the bias.  rel: j - i - offset of register row 0 of this half and this lane,
+// and sign +1 where the registers run over keys, -1 where they run over queries
+template <int SIGN>
+__device__ __forceinline__ void add_bias(f32x16& s, const float* line, float c, int rel, int D, int lo, int hi) {
+  if (lo >= D || hi <= -D) {   // the whole block is past the table's distance: one value
+    const float b = line[lo >= D ? 2 * D : 0];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int d = min(max(rel + SIGN * (8 * (r >> 2) + (r & 3)), -D), D) + D;
+      s[r] = fmaf(s[r], c, line[d]);
+    }
+  }
+}
+
+// XCD-aware block order: workgroups go to the 8 XCDs in turn; consecutive work items (the tiles that share
+// keys and values) go to one XCD, so that its L2 holds them once
+__device__ __forceinline__ int64_t work_item(int64_t items) {
+  const int64_t per = (items + 7) / 8;
+  return (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+}
+inline unsigned work_grid(int64_t items) { return (unsigned)((items + 7) / 8 * 8); }
+
+struct Launch {
+  hipError_t (*fwd)(const BtArgs&, hipStream_t);
+  hipError_t (*few)(const BtArgs&, hipStream_t);
+  hipError_t (*dq)(const BtArgs&, hipStream_t);
+  hipError_t (*dkv)(const BtArgs&, hipStream_t);
+};
+
+// dynamic LDS past 64 KiB has to be allowed once a device and kernel
+template <typename K>
+hipError_t allow_lds(K kernel, size_t bytes, std::atomic<bool> (&done)[64]) {
+  if (bytes <= 64 * 1024) return hipSuccess;
+  int dev = 0;
+  if (const hipError_t e = hipGetDevice(&dev)) return e;
+  if (dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
+    if (const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)) return e;
+    if (dev < 64) done[dev].store(true, std::memory_order_release);
+  }
+  return hipSuccess;
+}
+
+}  // namespace battn
+}  // namespace ggd

@@ -21,9 +21,11 @@ LIB_PATH = DIAG_LIB if os.environ.get("GGD_DIAG") == "1" else PRODUCT_LIB
 if os.environ.get("GGD_LIB"):
     LIB_PATH = os.path.abspath(os.environ["GGD_LIB"])
 SOURCES = ["ggd_kernels.hip", "ggd_fused.hip", "ggd_mega.hip", "ggd_rows.hip", "ggd_persist.hip", "ggd_encoder.hip", "ggd_train.hip", "ggd_chain.hip", "ggd_attn.hip", "ggd_long.hip",
-           "ggd_api.hip"]
+           "ggd_battn.hip", "ggd_battn_f32.hip", "ggd_resnorm.hip", "ggd_api.hip"]
+UNPACKED = ("ggd_battn.hip", "ggd_battn_f32.hip", "ggd_resnorm.hip")
 DIAG_SOURCES = ["ggd_diag.hip"]   # + ggd_api.hip again with -DGGD_DIAG
-HEADERS = ["ggd_kernels.h", "ggd_common.h", "ggd_chainlib.h", "ggd_fusedlib.h", "ggd_phases.h", "ggd_megasync.h", os.path.join("..", "..", "include", "ggd.h"),
+HEADERS = ["ggd_kernels.h", "ggd_common.h", "ggd_chainlib.h", "ggd_fusedlib.h", "ggd_phases.h", "ggd_megasync.h", "ggd_battn.h", "ggd_battn_kernels.h",
+           os.path.join("..", "..", "include", "ggd.h"),
            os.path.join("..", "..", "include", "ggd_train.h")]
 
 GGD_OK, GGD_IGNORED = 0, 1
@@ -48,6 +50,8 @@ EXPORTS = [
     "ggd_tr_mse", "ggd_tr_sumsq", "ggd_tr_sumsq_blocks", "ggd_tr_adamw", "ggd_tr_scale", "ggd_tr_scale_clamp",
     "ggd_tr_conv_fwd", "ggd_tr_conv_dgrad", "ggd_tr_conv_wgrad", "ggd_tr_im2col", "ggd_tr_col2im", "ggd_tr_batchnorm_fwd", "ggd_tr_batchnorm_bwd", "ggd_tr_image_channel_sum",
     "ggd_tr_channel_scale", "ggd_tr_pixel_shuffle", "ggd_tr_head_flatten", "ggd_enc_frontend",
+    "ggd_tr_resnorm_fwd", "ggd_tr_resnorm_bwd", "ggd_tr_resnorm_ws",
+    "ggd_tr_battn_fwd", "ggd_tr_battn_bwd", "ggd_tr_battn_ws",
 ]
 
 
@@ -66,6 +70,19 @@ class SampleArgs(ctypes.Structure):
         ("extras", ctypes.c_void_p), ("n_steps", ctypes.c_int32), ("use_graph", ctypes.c_int32),
         ("sync", ctypes.c_int32),
     ]
+
+
+class BattnArgs(ctypes.Structure):
+    """ggd_tr_battn_args (include/ggd_train.h)."""
+    _fields_ = (
+        [(n, ctypes.c_int32) for n in ("n", "heads", "kv_heads", "lq", "lk", "dk", "dtype")] + [("scale", ctypes.c_float)] +
+        [(n, ctypes.c_void_p) for n in ("q", "k", "v", "o")] +
+        [(n, ctypes.c_int64) for n in ("ldq", "bq", "ldk", "bk", "ldv", "bv", "ldo", "bo")] +
+        [("mask", ctypes.c_void_p), ("q_mask", ctypes.c_void_p), ("bmask", ctypes.c_int64), ("bq_mask", ctypes.c_int64),
+         ("table", ctypes.c_void_p), ("buckets", ctypes.c_void_p), ("n_buckets", ctypes.c_int32),
+         ("distance", ctypes.c_int32), ("offset", ctypes.c_int64)] +
+        [(n, ctypes.c_void_p) for n in ("stat", "o32", "dout", "dq", "dk_out", "dv", "dtable", "ws")] +
+        [("ws_bytes", ctypes.c_int64)])
 
 
 def _deps(path, seen=None):
@@ -104,8 +121,10 @@ def build(force=False, verbose=False):
     # costs issue slots (MI355X_MICROARCH.md, filler prices), and with it hipcc 7.2 clobbered a live
     # register of psk_kernel (the per-thread pose state) around the one-pass LayerNorm.
     flags = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-fno-slp-vectorize", "-Wno-unused-value", "-Wno-unused-result"]
+    # Packed f32 arithmetic off: some of its forms have given wrong results on gfx950 now and then.
+    no_packed = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     os.makedirs(os.path.join(PKG_DIR, "build"), exist_ok=True)
-    units = [(src, src.replace(".hip", ".o"), []) for src in SOURCES + DIAG_SOURCES]
+    units = [(src, src.replace(".hip", ".o"), no_packed if src in UNPACKED else []) for src in SOURCES + DIAG_SOURCES]
     units.append(("ggd_api.hip", "ggd_api_diag.o", ["-DGGD_DIAG"]))
     procs = []
     for src, obj_name, extra in units:  # one hipcc per translation unit, in parallel
@@ -203,6 +222,12 @@ def load():
         "ggd_tr_pixel_shuffle": (ctypes.c_int, [I32, I32, I32, I32, I32, VP, VP, I32, VP]),
         "ggd_tr_head_flatten": (ctypes.c_int, [I32, I32, I32, I32, VP, VP, I32, VP]),
         "ggd_enc_frontend": (ctypes.c_int, [CTX, VP, I32, VP, VP]),
+        "ggd_tr_resnorm_fwd": (ctypes.c_int, [I64, I32, I32, I32, F, F, VP, VP, VP, I64] + [VP] * 8),
+        "ggd_tr_resnorm_bwd": (ctypes.c_int, [I64, I32, I32, I32, F, F, VP, VP, VP, I64] + [VP] * 15 + [I64, VP]),
+        "ggd_tr_resnorm_ws": (I64, [I64, I32, I64, I32]),
+        "ggd_tr_battn_fwd": (ctypes.c_int, [P(BattnArgs), VP]),
+        "ggd_tr_battn_bwd": (ctypes.c_int, [P(BattnArgs), VP]),
+        "ggd_tr_battn_ws": (I64, [P(BattnArgs), I32]),
     }
     if LIB_PATH == DIAG_LIB or hasattr(lib, "ggd_diag"):  # (also a GGD_LIB diag variant, scripts/build_variant.sh)
         sig["ggd_diag"] = (ctypes.c_int, [CTX, I32, VP, I32, I32, VP])

@@ -1,0 +1,151 @@
+"""CPU tests of the decoder-block operators (…_amd/blocks.py): the buckets' plan, the C structure's layout, and every
+refusal, in Python and at the C entries, none of which launches anything."""
+import ctypes
+import importlib
+import math
+import os
+import subprocess
+
+import pytest
+import torch as th
+
+from tests.conftest import ROOT
+
+
+@pytest.fixture(scope="module")
+def native(pkg):
+    return importlib.import_module(pkg.__name__ + ".native")
+
+
+@pytest.mark.parametrize("n_buckets,most,both", [(32, 128, True), (32, 128, False), (4, 2, True), (2, 2, False), (20, 200, True), (64, 2047, True),
+                                                 (8, 5, True), (1024, 2000, True)])
+def test_relative_buckets(pkg, n_buckets, most, both):
+    """The definition over the reals: a distance at a border opens its bucket (its logarithm in 64 bits may not say so)."""
+    b = pkg.RelativeBuckets(n_buckets, most, both, device="cpu").buckets
+    side = n_buckets // 2 if both else n_buckets
+    near = side // 2
+    steps = side - near
+    assert b.dtype == th.int32 and b.numel() == 2 * most + 1
+    for d in range(-most, most + 1):
+        far = abs(d) if both else max(0, -d)
+        if far < near:
+            want = far
+        else:
+            x = math.log(far / near) / math.log(most / near) * steps
+            k = round(x) if abs(x - round(x)) < 1e-9 else math.floor(x)
+            if abs(x - round(x)) < 1e-9:   # a border in 64 bits: whole numbers decide
+                k = round(x) if far ** steps >= near ** (steps - round(x)) * most ** round(x) else round(x) - 1
+            want = near + min(k, steps - 1)
+        assert b[d + most] == want + (side if both and d > 0 else 0), d
+    assert b.min() == 0 and b.max() <= n_buckets - 1
+
+
+def test_relative_buckets_refusals(pkg):
+    for args in ((0, 8), (3, 8, True), (2, 8, True), (1, 8, False), (32, 8, True), (8, 2048, True), (1026, 2000, True), (32, 16, False)):
+        with pytest.raises(ValueError):
+            pkg.RelativeBuckets(*args, device="cpu")
+
+
+def test_operators_refuse_host_tensors(pkg):
+    """No CPU fallback."""
+    x = th.zeros(1, 2, 8)
+    with pytest.raises(ValueError):
+        pkg.cross_attention(x, x, x, 2)
+    with pytest.raises(ValueError):
+        pkg.relative_attention(x, x, x, 2, pkg.RelativeBuckets(8, 16, device="cpu"), th.zeros(8, 2))
+    with pytest.raises(ValueError):
+        pkg.residual_norm(x, x, (th.ones(8), None))
+    with pytest.raises(ValueError):
+        pkg.cross_attention(None, x, x, 2)
+
+
+def test_struct_layout_matches_header(native, tmp_path):
+    fields = [f for f, _ in native.BattnArgs._fields_]
+    src = tmp_path / "probe.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "ggd_train.h"\nint main(void) {\n' +
+                   "".join(f'printf("%zu\\n", offsetof(ggd_tr_battn_args, {f}));\n' for f in fields) +
+                   'printf("%zu\\n", sizeof(ggd_tr_battn_args));\nreturn 0;\n}\n')
+    exe = tmp_path / "probe"
+    subprocess.run(["gcc", "-std=c11", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [getattr(native.BattnArgs, f).offset for f in fields] + [ctypes.sizeof(native.BattnArgs)]
+
+
+def _battn(native, **over):
+    """Arguments in order for 2 clips, with addresses that a refused call never touches."""
+    at = 1 << 20
+    d = dict(n=2, heads=4, kv_heads=2, lq=3, lk=5, dk=16, dtype=1, scale=0.25, q=at, k=at, v=at, o=at, ldq=64, bq=192, ldk=32, bk=160, ldv=32,
+             bv=160, ldo=64, bo=192, stat=at, o32=at, dout=at, dq=at, dk_out=at, dv=at, ws=at, ws_bytes=1 << 40)
+    d.update(over)
+    return native.BattnArgs(**d)
+
+
+BAD = [dict(n=-1), dict(heads=0), dict(kv_heads=0), dict(heads=3), dict(lq=0), dict(lk=0), dict(dk=0), dict(dtype=2), dict(dtype=-1), dict(scale=0.0),
+       dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(ldq=-1), dict(bk=-8), dict(q=None), dict(k=None), dict(v=None),
+       dict(table=1 << 20), dict(buckets=1 << 20), dict(table=1 << 20, buckets=1 << 20, n_buckets=0, distance=4),
+       dict(table=1 << 20, buckets=1 << 20, n_buckets=4, distance=0)]
+UNSUPPORTED = [dict(dk=129), dict(lq=(1 << 28) + 1), dict(lk=(1 << 28) + 1), dict(table=1 << 20, buckets=1 << 20, n_buckets=1025, distance=4),
+               dict(table=1 << 20, buckets=1 << 20, n_buckets=8, distance=2048), dict(n=1 << 20, lq=1 << 20), dict(n=1, heads=64, kv_heads=1, lq=1 << 27)]
+
+
+def test_attention_entry_refusals(native):
+    lib = native.load()
+    call = lambda fn, **over: fn(ctypes.byref(_battn(native, **over)), None)
+    for over in BAD:
+        assert call(lib.ggd_tr_battn_fwd, **over) == -1, over
+        assert call(lib.ggd_tr_battn_bwd, **over) == -1, over
+    for over in UNSUPPORTED:
+        assert call(lib.ggd_tr_battn_fwd, **over) == -2, over
+        assert call(lib.ggd_tr_battn_bwd, **over) == -2, over
+        assert lib.ggd_tr_battn_ws(ctypes.byref(_battn(native, **over)), 1) == 0
+    assert lib.ggd_tr_battn_fwd(None, None) == -1 and lib.ggd_tr_battn_bwd(None, None) == -1 and lib.ggd_tr_battn_ws(None, 0) == 0
+    for over in (dict(o=None), dict(stat=None), dict(o32=None), dict(stat=(1 << 20) + 4)):
+        assert call(lib.ggd_tr_battn_fwd, **over) == -1, over
+    long = dict(lq=1, lk=100000)   # divided among blocks: needs its workspace
+    need = lib.ggd_tr_battn_ws(ctypes.byref(_battn(native, **long)), 0)
+    assert need > 0
+    for over in (dict(ws=None), dict(ws=(1 << 20) + 8), dict(ws_bytes=need - 1)):
+        assert call(lib.ggd_tr_battn_fwd, **long, **over) == -1, over
+    need = lib.ggd_tr_battn_ws(ctypes.byref(_battn(native)), 1)
+    for over in (dict(stat=None), dict(o32=None), dict(dout=None), dict(dq=None), dict(dk_out=None), dict(dv=None), dict(ws=None),
+                 dict(ws_bytes=need - 1), dict(dtable=1 << 20), dict(stat=(1 << 20) + 4)):
+        assert call(lib.ggd_tr_battn_bwd, **over) == -1, over
+    assert call(lib.ggd_tr_battn_fwd, n=0) == 0 and call(lib.ggd_tr_battn_bwd, n=0) == 0
+
+
+def test_residual_norm_entry_refusals(native):
+    lib = native.load()
+    at = 1 << 20
+    names = ("rows", "d", "dtype", "kind", "scale", "eps", "h", "y", "gate", "gate_rows", "post_g", "post_b", "pre_g", "pre_b")
+    good = dict(rows=6, d=8, dtype=0, kind=0, scale=1.0, eps=1e-5, h=at, y=at, gate=at, gate_rows=3, post_g=at, post_b=at, pre_g=at, pre_b=at)
+
+    def fwd(h_out=at, u=at, **over):
+        d = dict(good, **over)
+        return lib.ggd_tr_resnorm_fwd(*(d[k] for k in names), h_out, u, at, None)
+
+    outs = dict(stats=at, dh_out=at, du=at, dh=at, dy=at, dgate=at, d_post_g=at, d_post_b=at, d_pre_g=at, d_pre_b=at, ws=at, ws_bytes=1 << 40)
+
+    def bwd(**over):
+        d = dict(good, **{k: v for k, v in over.items() if k in good})
+        o = dict(outs, **{k: v for k, v in over.items() if k in outs})
+        return lib.ggd_tr_resnorm_bwd(*(d[k] for k in names), *o.values(), None)
+
+    for over in (dict(rows=-1), dict(d=0), dict(dtype=2), dict(kind=2), dict(eps=0.0), dict(eps=math.nan), dict(gate_rows=0), dict(gate_rows=4),
+                 dict(pre_g=None), dict(post_g=None), dict(h=None), dict(y=None)):
+        assert fwd(**over) == -1, over
+        assert bwd(**over) == -1, over
+    for over in (dict(h_out=None), dict(u=None)):
+        assert fwd(**over) == -1, over
+    for over in (dict(d=8193), dict(rows=1 << 32, gate=None)):
+        assert fwd(**over) == -2, over
+        assert bwd(**dict(over, dgate=None if "gate" in over else at)) == -2, over
+    for over in (dict(rows=0), *({k: None} for k in outs if k != "ws_bytes"), dict(gate=None), dict(pre_b=None), dict(post_b=None), dict(ws=at + 8),
+                 dict(ws_bytes=lib.ggd_tr_resnorm_ws(6, 8, 3, 1) - 1)):
+        assert bwd(**over) == -1, over
+    assert fwd(rows=0) == 0
+    assert lib.ggd_tr_resnorm_ws(0, 8, 1, 0) == 0 and lib.ggd_tr_resnorm_ws(6, 8, 4, 1) == 0 and lib.ggd_tr_resnorm_ws(6, 8193, 3, 1) == 0
+
+
+def test_entries_are_declared(native):
+    for name in ("ggd_tr_resnorm_fwd", "ggd_tr_resnorm_bwd", "ggd_tr_resnorm_ws", "ggd_tr_battn_fwd", "ggd_tr_battn_bwd", "ggd_tr_battn_ws"):
+        assert name in native.EXPORTS
