@@ -7,10 +7,10 @@ cd "$(dirname "$0")/.." || exit 1
 P=speech-driven-gesture-generation-using-transformer-based-denoising-diffusion-probabilistic-models_amd
 U=${3:-ggd_mega}
 mkdir -p ab /tmp/ggd_variant
-hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -fno-slp-vectorize -Wno-unused-value -Wno-unused-result $2 \
+hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -fno-slp-vectorize -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-value -Wno-unused-result $2 \
   -c $P/csrc/$U.hip -o /tmp/ggd_variant/${U}_$1.o || exit 1
 objs=""
-for s in ggd_kernels ggd_fused ggd_mega ggd_rows ggd_persist ggd_encoder ggd_train ggd_chain ggd_attn ggd_long ggd_api; do
+for s in ggd_kernels ggd_fused ggd_mega ggd_rows ggd_persist ggd_encoder ggd_train ggd_chain ggd_attn ggd_long ggd_battn ggd_battn_f32 ggd_resnorm ggd_api; do
   [ "$s" = "$U" ] || objs="$objs $P/build/$s.o"
 done
 hipcc --offload-arch=gfx950 -shared -fPIC $objs /tmp/ggd_variant/${U}_$1.o -o ab/libggd_$1.so && echo "ab/libggd_$1.so" || exit 1

@@ -13,6 +13,7 @@ A wrong shape, type or device raises ValueError before anything is launched.
 """
 import ctypes
 import math
+import struct
 
 import torch as th
 from torch.autograd.function import once_differentiable
@@ -21,11 +22,6 @@ from . import native
 
 MAX_HEAD_DIM, MAX_BUCKETS, MAX_DISTANCE, MAX_NORM_DIM = 128, 1024, 2047, 8192   # include/ggd_train.h
 _DTYPES = {th.float32: 0, th.bfloat16: 1}   # GGD_TR_F32, GGD_TR_BF16
-
-
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
 
 
 def _ok(rc, what):
@@ -39,16 +35,26 @@ def _p(t):
     return t.data_ptr() if t is not None else None
 
 
-def _stream(device):
-    return ctypes.c_void_p(th.cuda.current_stream(device).cuda_stream)
+def _call(fn, args, device, what):
+    """An entry point on the current stream of a device, which is the current one meanwhile."""
+    stream = th._C._cuda_getCurrentRawStream(device.index)
+    if device.index == th.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with th.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc != 0:
+        _ok(rc, what)
 
 
 def _tensors(what, first, rest):
     """All on the first one's GPU."""
-    _need(isinstance(first, th.Tensor) and first.is_cuda, f"{what}: the inputs have to be on a GPU device (no CPU fallback)")
-    for name, t in rest.items():
-        _need(isinstance(t, th.Tensor), f"{what}: {name} has to be a tensor")
-        _need(t.device == first.device, f"{what}: {name} is on {t.device}, the first input on {first.device}")
+    if not (isinstance(first, th.Tensor) and first.is_cuda):
+        raise ValueError(f"{what}: the inputs have to be on a GPU device (no CPU fallback)")
+    device = first.device
+    for name, t in rest:
+        if t is not None and not (isinstance(t, th.Tensor) and t.device == device):
+            raise ValueError(f"{what}: {name} has to be a tensor on {device}")
 
 
 def _workspace(nbytes, device):
@@ -72,11 +78,10 @@ class RelativeBuckets:
     def __init__(self, n_buckets=32, max_distance=128, both_sides=True, device="cuda"):
         n_buckets, max_distance = int(n_buckets), int(max_distance)
         side = n_buckets // 2 if both_sides else n_buckets
-        _need(1 <= n_buckets <= MAX_BUCKETS and not (both_sides and n_buckets % 2),
-              f"RelativeBuckets: n_buckets {n_buckets}: up to {MAX_BUCKETS}, even with both sides")
-        _need(side >= 2, f"RelativeBuckets: {n_buckets} buckets leave fewer than 2 for a side")
-        _need(side // 2 < max_distance <= MAX_DISTANCE,
-              f"RelativeBuckets: max_distance {max_distance}: more than {side // 2}, up to {MAX_DISTANCE}")
+        if not 1 <= n_buckets <= MAX_BUCKETS or (both_sides and n_buckets % 2) or side < 2:
+            raise ValueError(f"RelativeBuckets: n_buckets {n_buckets}: up to {MAX_BUCKETS}, at least 2 a side, even with both sides")
+        if not side // 2 < max_distance <= MAX_DISTANCE:
+            raise ValueError(f"RelativeBuckets: max_distance {max_distance}: more than {side // 2}, up to {MAX_DISTANCE}")
         self.n_buckets, self.max_distance, self.both_sides = n_buckets, max_distance, bool(both_sides)
         near, steps, of = side // 2, side - side // 2, []
         passed = 0
@@ -113,108 +118,103 @@ def _mask_rows(m):
     return m if m is None or m.stride(1) == 1 or m.shape[1] == 1 else m.contiguous()
 
 
-def _args(q, k, v, mask, q_mask, table, lut, geo):
+_PACK = struct.Struct("@" + "".join({ctypes.c_int32: "i", ctypes.c_float: "f", ctypes.c_int64: "q", ctypes.c_void_p: "P"}[t]
+                                    for _, t in native.BattnArgs._fields_)).pack   # ggd_tr_battn_args as bytes
+
+
+def _launch(entry, inputs, geo, o=None, stat=None, o32=None, grads=(None,) * 5):
+    """ggd_tr_battn_fwd or _bwd over its workspace.  grads: dout, dq, dk, dv, dtable."""
+    q, k, v, table, mask, q_mask, lut = inputs
     heads, kv_heads, scale, offset = geo
     n, lq, width = q.shape
-    a = native.BattnArgs(n=n, heads=heads, kv_heads=kv_heads, lq=lq, lk=k.shape[1], dk=width // heads, dtype=_DTYPES[q.dtype],
-                         scale=scale, q=_p(q), k=_p(k), v=_p(v), ldq=q.stride(1), bq=q.stride(0), ldk=k.stride(1),
-                         bk=k.stride(0), ldv=v.stride(1), bv=v.stride(0))
-    if mask is not None:
-        a.mask, a.bmask = _p(mask), mask.stride(0)
-    if q_mask is not None:
-        a.q_mask, a.bq_mask = _p(q_mask), q_mask.stride(0)
-    if table is not None:
-        a.table, a.buckets, a.n_buckets, a.distance = _p(table), _p(lut), table.shape[0], (lut.numel() - 1) // 2
-        a.offset = offset
-    return a
-
-
-def _attend(q, k, v, mask, q_mask, table, lut, geo, keep):
-    """o, and with keep what the backward pass needs: (stat, o32)."""
-    n, lq, width = q.shape
-    o = th.empty(n, lq, width, dtype=q.dtype, device=q.device)
-    if o.numel() == 0 or k.shape[1] == 0:
-        return o.zero_(), None, None
+    address = lambda t: t.data_ptr() if t is not None else 0
+    head = (n, heads, kv_heads, lq, k.shape[1], width // heads, _DTYPES[q.dtype], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), address(o),
+            q.stride(1), q.stride(0), k.stride(1), k.stride(0), v.stride(1), v.stride(0), width, lq * width,
+            address(mask), address(q_mask), 0 if mask is None else mask.stride(0), 0 if q_mask is None else q_mask.stride(0),
+            address(table), address(lut), *((0, 0, 0) if table is None else (table.shape[0], lut.shape[0] // 2, offset)),
+            address(stat), address(o32), *map(address, grads))
     lib = native.load()
-    a = _args(q, k, v, mask, q_mask, table, lut, geo)
-    a.o, a.ldo, a.bo = _p(o), width, lq * width
+    backward = entry == "ggd_tr_battn_bwd"
+    nbytes = lib.ggd_tr_battn_ws(_PACK(*head, 0, 0), backward)
+    ws = _workspace(nbytes, q.device)
+    _call(getattr(lib, entry), (_PACK(*head, address(ws), nbytes),), q.device, "attention backward" if backward else "attention")
+
+
+def _attend(inputs, geo, keep):
+    """o, and with keep what the backward pass needs: (stat, o32)."""
+    q = inputs[0]
+    n, lq, width = q.shape
+    o = th.empty((n, lq, width), dtype=q.dtype, device=q.device)
+    if o.numel() == 0 or inputs[1].shape[1] == 0:
+        return o.zero_(), None, None
     stat = o32 = None
     if keep:
-        stat = th.empty(n, geo[0], lq, 2, dtype=th.float32, device=q.device)
-        o32 = o if q.dtype == th.float32 else th.empty(n, lq, width, dtype=th.float32, device=q.device)
-        a.stat, a.o32 = _p(stat), _p(o32)
-    a.ws_bytes = lib.ggd_tr_battn_ws(ctypes.byref(a), 0)
-    ws = _workspace(a.ws_bytes, q.device)
-    a.ws = _p(ws)
-    with th.cuda.device(q.device):
-        _ok(lib.ggd_tr_battn_fwd(ctypes.byref(a), _stream(q.device)), "attention")
+        stat = th.empty((n, geo[0], lq, 2), dtype=th.float32, device=q.device)
+        o32 = o if q.dtype == th.float32 else th.empty((n, lq, width), dtype=th.float32, device=q.device)
+    _launch("ggd_tr_battn_fwd", inputs, geo, o, stat, o32)
     return o, stat, o32
 
 
 class _Battn(th.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, mask, q_mask, lut, geo):
-        o, stat, o32 = _attend(q, k, v, mask, q_mask, table, lut, geo, True)
-        ctx.save_for_backward(q, k, v, table, mask, q_mask, lut, stat, o32)
+        inputs = (q, k, v, table, mask, q_mask, lut)
+        o, stat, o32 = _attend(inputs, geo, True)
+        ctx.save_for_backward(*inputs, stat, o32)
         ctx.geo = geo
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, table, mask, q_mask, lut, stat, o32 = ctx.saved_tensors
-        new = lambda t, dtype: th.empty(t.shape, dtype=dtype, device=t.device)
-        dq, dk, dv = new(q, q.dtype), new(k, k.dtype), new(v, v.dtype)
-        dtable = new(table, table.dtype) if table is not None and ctx.needs_input_grad[3] else None
+        *inputs, stat, o32 = ctx.saved_tensors
+        q, k, v, table = inputs[:4]
+        new = lambda t: th.empty(t.shape, dtype=t.dtype, device=t.device)
+        dq, dk, dv = new(q), new(k), new(v)
+        dtable = new(table) if table is not None and ctx.needs_input_grad[3] else None
         if stat is None:   # no query, or no key
             return (*(t if t is None else t.zero_() for t in (dq, dk, dv, dtable)), None, None, None, None)
         do = do.contiguous()
-        lib = native.load()
-        a = _args(q, k, v, mask, q_mask, table, lut, ctx.geo)
-        a.stat, a.o32, a.dout, a.dq, a.dk_out, a.dv, a.dtable = (_p(t) for t in (stat, o32, do, dq, dk, dv, dtable))
-        a.ws_bytes = lib.ggd_tr_battn_ws(ctypes.byref(a), 1)
-        ws = _workspace(a.ws_bytes, q.device)
-        a.ws = _p(ws)
-        with th.cuda.device(q.device):
-            _ok(lib.ggd_tr_battn_bwd(ctypes.byref(a), _stream(q.device)), "attention backward")
+        _launch("ggd_tr_battn_bwd", inputs, ctx.geo, None, stat, o32, (do, dq, dk, dv, dtable))
         return dq, dk, dv, dtable, None, None, None, None
 
 
 def _attention(what, q, k, v, heads, kv_heads, scale, mask, q_mask, buckets=None, table=None, offset=0):
-    rest = {"k": k, "v": v}
-    rest.update({name: t for name, t in (("mask", mask), ("q_mask", q_mask), ("table", table)) if t is not None})
-    _tensors(what, q, rest)
+    _tensors(what, q, (("k", k), ("v", v), ("mask", mask), ("q_mask", q_mask), ("table", table)))
     heads = int(heads)
     kv_heads = heads if kv_heads is None else int(kv_heads)
-    _need(heads >= 1 and kv_heads >= 1 and heads % kv_heads == 0, f"{what}: {heads} heads over {kv_heads} kv heads")
-    _need(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, f"{what}: q, k and v have to be (n, L, heads dk)")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{what}: {heads} heads over {kv_heads} kv heads")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"{what}: q, k and v have to be (n, L, heads dk)")
     n, lq, width = q.shape
-    _need(width % heads == 0 and width > 0, f"{what}: q rows of {width} elements are not {heads} heads")
+    if width % heads or not 1 <= width // heads <= MAX_HEAD_DIM:
+        raise ValueError(f"{what}: q rows of {width} elements are not {heads} heads of 1 to {MAX_HEAD_DIM}")
     dk = width // heads
-    _need(dk <= MAX_HEAD_DIM, f"{what}: heads of {dk} elements: up to {MAX_HEAD_DIM}")
-    _need(tuple(k.shape) == tuple(v.shape) and k.shape[0] == n and k.shape[2] == kv_heads * dk,
-          f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} have to be ({n}, Lk, {kv_heads * dk})")
-    _need(q.dtype in _DTYPES and k.dtype == q.dtype and v.dtype == q.dtype,
-          f"{what}: q, k and v have to be of one type, float32 or bfloat16")
     lk = k.shape[1]
+    if k.shape != (n, lk, kv_heads * dk) or v.shape != k.shape:
+        raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} have to be ({n}, Lk, {kv_heads * dk})")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{what}: q, k and v have to be of one type, float32 or bfloat16")
     for name, m, length in (("mask", mask, lk), ("q_mask", q_mask, lq)):
-        _need(m is None or (m.dtype == th.bool and tuple(m.shape) == (n, length)),
-              f"{what}: {name} has to be ({n}, {length}) truth values")
+        if m is not None and (m.dtype != th.bool or m.shape != (n, length)):
+            raise ValueError(f"{what}: {name} has to be ({n}, {length}) truth values")
     scale = 1.0 / math.sqrt(dk) if scale is None else float(scale)
-    _need(0.0 < scale <= 1e30, f"{what}: scale {scale} has to be positive")
+    if not 0.0 < scale <= 1e30:
+        raise ValueError(f"{what}: scale {scale} has to be positive")
     lut = None
     if table is not None:
-        _need(isinstance(buckets, RelativeBuckets), f"{what}: buckets has to be a RelativeBuckets")
-        _need(table.dtype == th.float32 and tuple(table.shape) == (buckets.n_buckets, heads),
-              f"{what}: table has to be ({buckets.n_buckets}, {heads}) in float32")
+        if not isinstance(buckets, RelativeBuckets):
+            raise ValueError(f"{what}: buckets has to be a RelativeBuckets")
+        if table.dtype != th.float32 or table.shape != (buckets.n_buckets, heads):
+            raise ValueError(f"{what}: table has to be ({buckets.n_buckets}, {heads}) in float32")
         table = table.contiguous()
         lut = buckets.on(q.device)
-    q, k, v, mask, q_mask = _rows(q), _rows(k), _rows(v), _mask_rows(mask), _mask_rows(q_mask)
-    offset = max(-(1 << 62), min(1 << 62, int(offset)))
-    geo = (heads, kv_heads, scale, offset)
-    if th.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
-        return _Battn.apply(q, k, v, table, mask, q_mask, lut, geo)
-    return _attend(q, k, v, mask, q_mask, table, lut, geo, False)[0]
+    inputs = (_rows(q), _rows(k), _rows(v), table, _mask_rows(mask), _mask_rows(q_mask), lut)
+    geo = (heads, kv_heads, scale, max(-(1 << 62), min(1 << 62, int(offset))))
+    if th.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)):
+        return _Battn.apply(*inputs, geo)
+    return _attend(inputs, geo, False)[0]
 
 
 def cross_attention(q, k, v, heads, kv_heads=None, scale=None, mask=None, q_mask=None):
@@ -240,7 +240,8 @@ def relative_attention(q, k, v, heads, buckets, table, offset=0, kv_heads=None, 
     -inf forbids its positions.  offset: the position of query row 0 where key row 0 has position 0 -- 0
     over a whole sequence, Lk - Lq for a stream's newest frames over all frames so far.
     """
-    _need(table is not None, "relative_attention: table has to be a tensor")
+    if table is None:
+        raise ValueError("relative_attention: table has to be a tensor")
     return _attention("relative_attention", q, k, v, heads, kv_heads, scale, mask, q_mask, buckets, table, offset)
 
 
@@ -256,11 +257,9 @@ def _norm_forward(h, y, gate, weights, geo, keep):
     stats = None
     if rows:
         stats = th.empty(4, rows, dtype=th.float32, device=h.device) if keep else None
-        post_g, post_b, pre_g, pre_b = weights
-        with th.cuda.device(h.device):
-            _ok(native.load().ggd_tr_resnorm_fwd(rows, d, _DTYPES[h.dtype], kind, scale, eps, _p(h), _p(y), _p(gate),
-                                                 gate_rows, _p(post_g), _p(post_b), _p(pre_g), _p(pre_b), _p(h_out),
-                                                 _p(u), _p(stats), _stream(h.device)), "residual_norm")
+        _call(native.load().ggd_tr_resnorm_fwd,
+              (rows, d, _DTYPES[h.dtype], kind, scale, eps, _p(h), _p(y), _p(gate), gate_rows, *map(_p, weights), _p(h_out), _p(u), _p(stats)),
+              h.device, "residual_norm")
     return h_out, u, stats
 
 
@@ -285,11 +284,9 @@ class _ResidualNorm(th.autograd.Function):
         lib = native.load()
         nbytes = lib.ggd_tr_resnorm_ws(rows, d, gate_rows, int(gate is not None))
         ws = _workspace(nbytes, h.device)
-        with th.cuda.device(h.device):
-            _ok(lib.ggd_tr_resnorm_bwd(rows, d, _DTYPES[h.dtype], kind, scale, eps, _p(h), _p(y), _p(gate), gate_rows,
-                                       _p(post_g), _p(post_b), _p(pre_g), _p(pre_b), _p(stats), _p(dh_out), _p(du),
-                                       _p(dh), _p(dy), _p(dgate), *(_p(w) for w in weights), _p(ws), nbytes,
-                                       _stream(h.device)), "residual_norm backward")
+        _call(lib.ggd_tr_resnorm_bwd,
+              (rows, d, _DTYPES[h.dtype], kind, scale, eps, _p(h), _p(y), _p(gate), gate_rows, _p(post_g), _p(post_b), _p(pre_g), _p(pre_b),
+               _p(stats), _p(dh_out), _p(du), _p(dh), _p(dy), _p(dgate), *map(_p, weights), _p(ws), nbytes), h.device, "residual_norm backward")
         return (dh, dy, dgate, *weights, None)
 
 
@@ -297,8 +294,8 @@ def _gate_rows(gate, shape):
     """Rows of h that share a row of the gate, and the gate as it is read: leading dimensions of h, then ones,
     then d; any other shape that broadcasts is expanded."""
     rows = math.prod(shape[:-1])
-    _need(gate.dim() <= len(shape) and gate.dim() >= 1 and all(g in (1, s) for g, s in zip(gate.shape[::-1], shape[::-1])),
-          f"residual_norm: gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
+    if not 1 <= gate.dim() <= len(shape) or any(g not in (1, s) for g, s in zip(gate.shape[::-1], shape[::-1])):
+        raise ValueError(f"residual_norm: gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
     full = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
     at = len(shape) - 1
     while at > 0 and full[at - 1] == 1:
@@ -319,33 +316,41 @@ def residual_norm(h, y, pre, post=None, gate=None, scale=1.0, kind="layer", eps=
     type.  Gradients reach h, y, gate and the weights.
     """
     what = "residual_norm"
-    weights = {}
     for name, pair in (("pre", pre), ("post", post)):
-        if pair is None and name == "post":
-            pair = (None, None)
-        _need(isinstance(pair, (tuple, list)) and len(pair) == 2, f"{what}: {name} has to be (weight, bias)")
-        weights[name + " weight"], weights[name + " bias"] = pair
-    _need(weights["pre weight"] is not None, f"{what}: pre needs a weight")
-    _need(weights["post bias"] is None or weights["post weight"] is not None, f"{what}: post has a bias and no weight")
-    given = {name: t for name, t in weights.items() if t is not None}
-    _tensors(what, h, dict(given, y=y, **({} if gate is None else {"gate": gate})))
-    _need(kind in _KINDS, f"{what}: kind {kind!r}: layer or rms")
-    _need(h.dim() >= 1 and tuple(h.shape) == tuple(y.shape), f"{what}: h {tuple(h.shape)} and y {tuple(y.shape)} have to be of one shape")
-    _need(h.dtype in _DTYPES and y.dtype == h.dtype and (gate is None or gate.dtype == h.dtype),
-          f"{what}: h, y and gate have to be of one type, float32 or bfloat16")
-    d = h.shape[-1]
-    _need(1 <= d <= MAX_NORM_DIM, f"{what}: rows of {d} elements: 1 to {MAX_NORM_DIM}")
-    for name, t in given.items():
-        _need(t.dtype == th.float32 and tuple(t.shape) == (d,), f"{what}: {name} has to be ({d},) in float32")
+        if not (isinstance(pair, (tuple, list)) and len(pair) == 2 or name == "post" and pair is None):
+            raise ValueError(f"{what}: {name} has to be (weight, bias)")
+    pre_g, pre_b = pre
+    post_g, post_b = (None, None) if post is None else post
+    if pre_g is None or (post_g is None and post_b is not None):
+        raise ValueError(f"{what}: a norm needs a weight")
+    _tensors(what, h, (("y", y), ("gate", gate), ("a weight of pre", pre_g), ("a bias of pre", pre_b), ("a weight of post", post_g),
+                       ("a bias of post", post_b)))
+    if kind not in _KINDS:
+        raise ValueError(f"{what}: kind {kind!r}: layer or rms")
+    shape = h.shape
+    if h.dim() < 1 or y.shape != shape:
+        raise ValueError(f"{what}: h {tuple(shape)} and y {tuple(y.shape)} have to be of one shape")
+    if h.dtype not in _DTYPES or y.dtype != h.dtype or (gate is not None and gate.dtype != h.dtype):
+        raise ValueError(f"{what}: h, y and gate have to be of one type, float32 or bfloat16")
+    d = shape[-1]
+    if not 1 <= d <= MAX_NORM_DIM:
+        raise ValueError(f"{what}: rows of {d} elements: 1 to {MAX_NORM_DIM}")
+    weights = [post_g, post_b, pre_g, pre_b]
+    grad = h.requires_grad or y.requires_grad or (gate is not None and gate.requires_grad)
+    for i, t in enumerate(weights):
+        if t is not None:
+            if t.dtype != th.float32 or t.shape != (d,):
+                raise ValueError(f"{what}: weights and biases have to be ({d},) in float32")
+            grad = grad or t.requires_grad
+            weights[i] = t.contiguous()
     scale, eps = float(scale), float(eps)
-    _need(math.isfinite(scale) and math.isfinite(eps) and eps > 0, f"{what}: scale {scale} has to be finite, eps {eps} positive")
-    rows = h.numel() // d
+    if not (math.isfinite(scale) and math.isfinite(eps) and eps > 0):
+        raise ValueError(f"{what}: scale {scale} has to be finite, eps {eps} positive")
     gate_rows = 1
     if gate is not None:
-        gate_rows, gate = _gate_rows(gate, tuple(h.shape))
+        gate_rows, gate = _gate_rows(gate, shape)
     h, y = h.contiguous(), y.contiguous()
-    order = [weights[k] if weights[k] is None else weights[k].contiguous() for k in ("post weight", "post bias", "pre weight", "pre bias")]
-    geo = (rows, d, gate_rows, _KINDS[kind], scale, eps)
-    if th.is_grad_enabled() and any(t is not None and t.requires_grad for t in (h, y, gate, *order)):
-        return _ResidualNorm.apply(h, y, gate, *order, geo)
-    return _norm_forward(h, y, gate, order, geo, False)[:2]
+    geo = (h.numel() // d, d, gate_rows, _KINDS[kind], scale, eps)
+    if grad and th.is_grad_enabled():
+        return _ResidualNorm.apply(h, y, gate, *weights, geo)
+    return _norm_forward(h, y, gate, weights, geo, False)[:2]

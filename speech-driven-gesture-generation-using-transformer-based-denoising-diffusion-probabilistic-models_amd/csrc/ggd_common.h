@@ -243,8 +243,8 @@ __device__ __forceinline__ float group_max(float v) {
 }
 
 // LayerNorm statistics of rows held by 4 consecutive lanes, N float4 of the row per lane (two-pass:
-// mean, then the centred sum of squares), on packed f32 pairs (v_pk_add / v_pk_mul / v_pk_fma_f32,
-// half the instructions of the scalar form) with explicit fma so that the contraction cannot
+// mean, then the centred sum of squares), on f32 pairs (two scalar operations
+// each: the build has packed f32 arithmetic off) with explicit fma so that the contraction cannot
 // depend on the call site: shared by gemm_kernel's PRO_LN prologue, the row-block chains and the
 // long-clip loop, which must agree bit for bit.  k = the row length.
 template <int N>

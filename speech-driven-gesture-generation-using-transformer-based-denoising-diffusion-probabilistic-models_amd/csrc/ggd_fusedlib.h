@@ -437,9 +437,9 @@ __device__ __forceinline__ void ln_apply(const float* Hs, int L, const float2* s
 // the T image (stride SXI).  Each row is held by 8 lanes, 32 values each, in registers: mean,
 // centred variance (two-pass, as torch) and the normalised output need no LDS round trip and no
 // barrier between them.  Rows L .. NR - 1 are written as zeros.  The per-value arithmetic runs on
-// packed f32 pairs (v_pk_add / v_pk_fma / v_pk_mul_f32) and bf16 pairs are converted with one
-// v_cvt_pk_bf16_f32: half the VALU instructions of the scalar form (the LN segments are
-// instruction-bound on the 5 waves that hold the 40 rows; measured 0.9 us per LN before).
+// f32 pairs (two scalar operations each: the build has packed f32 arithmetic off) and bf16 pairs are
+// converted with one v_cvt_pk_bf16_f32 (the LN segments are instruction-bound on the 5 waves that
+// hold the 40 rows).
 template <typename T, int NT, int NR, int SXI = Frag<T>::SX>
 __device__ __forceinline__ void ln_rows(const float* Hs, int L, T* img, int tid = ltid()) {
   typedef float f2 __attribute__((ext_vector_type(2)));
@@ -735,7 +735,7 @@ __device__ __forceinline__ void fattn(unsigned char* att, int Lq, int Lk, float 
   }
   // softmax in the base-2 domain: exp(scale s - m) = exp2(scale log2(e) s - m'), one v_exp_f32
   // per score (and one v_rcp_f32 per row) instead of the range-reduced library expf / division
-  // The lane's 4 rows run as two packed f32 pairs (rows 0-1, 2-3: v_pk_mul / v_pk_add_f32) for
+  // The lane's 4 rows run as two f32 pairs (rows 0-1, 2-3) for
   // the scaling, the sums and the normalisation; per element the operations and their order are
   // the scalar ones.  A masked key is -inf after the scaling, so its exp2 is 0 without a select.
   typedef float f2 __attribute__((ext_vector_type(2)));

@@ -22,7 +22,6 @@ if os.environ.get("GGD_LIB"):
     LIB_PATH = os.path.abspath(os.environ["GGD_LIB"])
 SOURCES = ["ggd_kernels.hip", "ggd_fused.hip", "ggd_mega.hip", "ggd_rows.hip", "ggd_persist.hip", "ggd_encoder.hip", "ggd_train.hip", "ggd_chain.hip", "ggd_attn.hip", "ggd_long.hip",
            "ggd_battn.hip", "ggd_battn_f32.hip", "ggd_resnorm.hip", "ggd_api.hip"]
-UNPACKED = ("ggd_battn.hip", "ggd_battn_f32.hip", "ggd_resnorm.hip")
 DIAG_SOURCES = ["ggd_diag.hip"]   # + ggd_api.hip again with -DGGD_DIAG
 HEADERS = ["ggd_kernels.h", "ggd_common.h", "ggd_chainlib.h", "ggd_fusedlib.h", "ggd_phases.h", "ggd_megasync.h", "ggd_battn.h", "ggd_battn_kernels.h",
            os.path.join("..", "..", "include", "ggd.h"),
@@ -120,11 +119,14 @@ def build(force=False, verbose=False):
     # -fno-slp-vectorize: no packed-f32 (v_pk_*_f32) code from the SLP vectorizer.  Beside MFMAs it
     # costs issue slots (MI355X_MICROARCH.md, filler prices), and with it hipcc 7.2 clobbered a live
     # register of psk_kernel (the per-thread pose state) around the one-pass LayerNorm.
-    flags = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-fno-slp-vectorize", "-Wno-unused-value", "-Wno-unused-result"]
-    # Packed f32 arithmetic off: some of its forms have given wrong results on gfx950 now and then.
-    no_packed = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    # -packed-fp32-ops: no packed f32 arithmetic from anywhere else either (explicit two-element vectors run as scalar
+    # pairs): some of its forms have given wrong results on gfx950 now and then, with no error.  hipcc's host pass
+    # says that it does not know the feature.  The long-clip loop is 1.8 % slower for it (145.3 -> 147.9 ms over
+    # 32 clips), the other loops stay inside the spread.
+    flags = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-fno-slp-vectorize", "-Xclang", "-target-feature",
+             "-Xclang", "-packed-fp32-ops", "-Wno-unused-value", "-Wno-unused-result"]
     os.makedirs(os.path.join(PKG_DIR, "build"), exist_ok=True)
-    units = [(src, src.replace(".hip", ".o"), no_packed if src in UNPACKED else []) for src in SOURCES + DIAG_SOURCES]
+    units = [(src, src.replace(".hip", ".o"), []) for src in SOURCES + DIAG_SOURCES]
     units.append(("ggd_api.hip", "ggd_api_diag.o", ["-DGGD_DIAG"]))
     procs = []
     for src, obj_name, extra in units:  # one hipcc per translation unit, in parallel
@@ -225,9 +227,10 @@ def load():
         "ggd_tr_resnorm_fwd": (ctypes.c_int, [I64, I32, I32, I32, F, F, VP, VP, VP, I64] + [VP] * 8),
         "ggd_tr_resnorm_bwd": (ctypes.c_int, [I64, I32, I32, I32, F, F, VP, VP, VP, I64] + [VP] * 15 + [I64, VP]),
         "ggd_tr_resnorm_ws": (I64, [I64, I32, I64, I32]),
-        "ggd_tr_battn_fwd": (ctypes.c_int, [P(BattnArgs), VP]),
-        "ggd_tr_battn_bwd": (ctypes.c_int, [P(BattnArgs), VP]),
-        "ggd_tr_battn_ws": (I64, [P(BattnArgs), I32]),
+        # (a BattnArgs by reference, or its bytes)
+        "ggd_tr_battn_fwd": (ctypes.c_int, [VP, VP]),
+        "ggd_tr_battn_bwd": (ctypes.c_int, [VP, VP]),
+        "ggd_tr_battn_ws": (I64, [VP, I32]),
     }
     if LIB_PATH == DIAG_LIB or hasattr(lib, "ggd_diag"):  # (also a GGD_LIB diag variant, scripts/build_variant.sh)
         sig["ggd_diag"] = (ctypes.c_int, [CTX, I32, VP, I32, I32, VP])
