@@ -182,7 +182,8 @@ typedef struct ggd_tr_battn_args {
   const void* dout;
   void *dq, *dk_out, *dv;
   float* dtable;
-  void* ws;                                /* ggd_tr_battn_ws bytes, 16-byte aligned, this call's alone until it has run */
+  void* ws;                                /* ggd_tr_battn_ws bytes (of the same arguments), 16-byte aligned, this call's
+                                            * alone until it has run */
   int64_t ws_bytes;
 } ggd_tr_battn_args;
 int ggd_tr_battn_fwd(const ggd_tr_battn_args* args, void* stream);

@@ -41,8 +41,9 @@ struct BtArgs : ggd_tr_battn_args {
   int group;       // query heads of a kv head
   int off;         // offset, clamped (past the table's distance on either side all is one bucket)
   int splits;      // parts of the streamed axis (few, dq, dkv)
-  int vec;         // rows are 16-byte aligned and dk a multiple of 16 bytes
   int vec_o;       // the written rows take 4-element stores
+  int64_t hq, hk;  // elements between the heads of a row of q and dout, of k and v (dk, or what it is padded to)
+  int64_t lddo;    // elements between rows of dout
   float c;         // scale log2(e): scores are held in log2 units
   float* part;     // partial results of the splits
   float* delta;    // [n][heads][lq]
@@ -85,31 +86,76 @@ __device__ __forceinline__ int mask_byte(const uint8_t* mask, int row0, int rows
   return mask ? mask[r] : 1;
 }
 
+// unit u of a row: zeros past dk.  (Rows are 16-byte aligned and dk whole units: others are packed first.)
 template <typename T>
-__device__ __forceinline__ uint4 load_unit(const T* __restrict__ row, int u, int dk, bool vec) {
+__device__ __forceinline__ uint4 load_unit(const T* __restrict__ row, int u, int dk) {
   constexpr int EPU = 16 / sizeof(T);
-  const int c = u * EPU;
-  if (vec) return c < dk ? *(const uint4*)(row + c) : make_uint4(0, 0, 0, 0);
-  union { T e[EPU]; uint4 v; } x;
-  x.v = make_uint4(0, 0, 0, 0);
-#pragma unroll
-  for (int i = 0; i < EPU; ++i)
-    if (c + i < dk) x.e[i] = row[c + i];
-  return x.v;
+  return u * EPU < dk ? *(const uint4*)(row + u * EPU) : make_uint4(0, 0, 0, 0);
 }
 
-// One tile of rows on its way from memory to an LDS image: THREADS threads hold N units each.  Rows
-// whose bit is clear are not read; they are zeros in the image, whatever memory holds there.
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+// a buffer over the memory from a wave-uniform address on; the offset BT_OUT lies past its end and reads as zero
+constexpr int BT_OUT = INT32_MIN;
+__device__ __forceinline__ i32x4 buffer_at(const void* p) {
+  const uint64_t at = (uint64_t)p;
+  return i32x4{(int)__builtin_amdgcn_readfirstlane((int)at), (int)(__builtin_amdgcn_readfirstlane((int)(at >> 32)) & 0xFFFF), 0x7FFFFFFF, 0x00020000};
+}
+
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// One tile of rows from memory into an LDS image, straight (buffer loads to LDS: no registers, nothing for the VALU).
+// Thread t of instruction i fills unit t + i THREADS of the image, and reads the row's unit that swz puts there.  Rows whose
+// bit is clear are not read: their offset lies past the buffer's end, and zeros go into the image.
+//   The loads are issued by asm (the builtin makes the compiler wait for them at the next LDS access); they have
+// landed after tile_ready().
+template <typename T, int DK, int ROWS>
+struct Tile {
+  static constexpr int UPR = Img<T, DK>::UPR, N = ROWS * UPR / 256, STEP = 256 / UPR;   // instructions; rows between them
+  static_assert(ROWS * UPR % 256 == 0, "whole units a thread");
+  static constexpr int KINDS = STEP % 16 ? 2 : 1;   // (f32, 128: rows 8 apart have another swz)
+  int row;          // of instruction 0
+  int off[KINDS];   // byte offset of its unit, BT_OUT past dk
+  __device__ __forceinline__ void start(int64_t ld, int dk) {
+    const int t = threadIdx.x;
+    row = t / UPR;
+#pragma unroll
+    for (int k = 0; k < KINDS; ++k) {
+      const int u = (t % UPR) ^ Img<T, DK>::swz(row + k * STEP);
+      off[k] = u * Img<T, DK>::EPU < dk ? (int)(row * ld * (int64_t)sizeof(T)) + u * 16 : BT_OUT;
+    }
+  }
+  __device__ __forceinline__ void load(const T* base, int64_t ld, uint64_t bits, const uint4* img) const {
+    const i32x4 rs = buffer_at(base);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(img) + (threadIdx.x >> 6) * 1024);
+    const int step = (int)(STEP * ld * (int64_t)sizeof(T));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int o = off[i % KINDS];
+      issue(rs, (bits >> (row + i * STEP)) & 1 && o != BT_OUT ? o + i * step : BT_OUT, at + i * 4096);
+    }
+  }
+  // (five wait states: the descriptor and the address may come from the VALU's readfirstlane)
+  static __device__ __forceinline__ void issue(i32x4 rs, int offset, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(rs) : "memory");
+  }
+};
+
+// the block's loads have landed in LDS, and every wave is past its last reads of the other buffer
+__device__ __forceinline__ void tile_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// the same through registers, for a wave alone (bt_few_kernel): the loads stay in flight while it works
 template <typename T, int DK, int ROWS, int THREADS>
 struct Stage {
   static constexpr int UPR = Img<T, DK>::UPR, N = ROWS * UPR / THREADS;
   static_assert(ROWS * UPR % THREADS == 0, "whole units a thread");
   uint4 x[N];
-  __device__ __forceinline__ void load(const T* __restrict__ base, int64_t ld, uint64_t bits, int dk, bool vec, int t) {
+  __device__ __forceinline__ void load(const T* __restrict__ base, int64_t ld, uint64_t bits, int dk, int t) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = t + i * THREADS, r = e / UPR, u = e % UPR;
-      x[i] = (bits >> r) & 1 ? load_unit(base + r * ld, u, dk, vec) : make_uint4(0, 0, 0, 0);
+      x[i] = (bits >> r) & 1 ? load_unit(base + r * ld, u, dk) : make_uint4(0, 0, 0, 0);
     }
   }
   __device__ __forceinline__ void store(uint4* img, int t) const {
@@ -130,10 +176,10 @@ template <typename T, int DK>
 struct Frag {
   static constexpr int N = Img<T, DK>::UPR / 2;
   uint4 x[N];
-  __device__ __forceinline__ void load(const T* __restrict__ row, int dk, bool vec, bool there) {
+  __device__ __forceinline__ void load(const T* __restrict__ row, int dk, bool there) {
     const int h = lane_id() >> 5;
 #pragma unroll
-    for (int s = 0; s < N; ++s) x[s] = there ? load_unit(row, 2 * s + h, dk, vec) : make_uint4(0, 0, 0, 0);
+    for (int s = 0; s < N; ++s) x[s] = there ? load_unit(row, 2 * s + h, dk) : make_uint4(0, 0, 0, 0);
   }
 };
 
@@ -291,6 +337,7 @@ __device__ __forceinline__ int64_t work_item(int64_t items) {
 inline unsigned work_grid(int64_t items) { return (unsigned)((items + 7) / 8 * 8); }
 
 struct Launch {
+  hipError_t (*pack)(const BtArgs&, const void* src, int64_t ld, int64_t b, int rows, int heads, void* dst, hipStream_t);
   hipError_t (*fwd)(const BtArgs&, hipStream_t);
   hipError_t (*few)(const BtArgs&, hipStream_t);
   hipError_t (*dq)(const BtArgs&, hipStream_t);

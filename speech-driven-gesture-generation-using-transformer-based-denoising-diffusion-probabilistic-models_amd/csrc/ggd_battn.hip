@@ -36,10 +36,24 @@ int prepare(const ggd_tr_battn_args* in, BtArgs& a) {
 
 size_t esize(const BtArgs& a) { return a.dtype == GGD_TR_F32 ? 4 : 2; }
 
-// 16-byte loads of rows: every row starts at a multiple of 16 bytes and holds whole units
-bool vec_rows(const BtArgs& a, const void* p, int64_t ld, int64_t b) {
+// The kernels read rows in 16-byte units, and a tile of 64 rows by 32-bit offsets: rows that do not start at a multiple of 16
+// bytes, hold other than whole units or lie too far apart are packed first (one more pass over them, without a limit on strides).
+constexpr int64_t BT_MAX_LD = 1 << 22;
+bool whole_rows(const BtArgs& a, const void* p, int64_t ld, int64_t b) {
   const int64_t per = 16 / (int64_t)esize(a);
-  return aligned(p, 16) && ld % per == 0 && b % per == 0 && a.dk % per == 0;
+  return aligned(p, 16) && ld % per == 0 && ld <= BT_MAX_LD && b % per == 0 && a.dk % per == 0;
+}
+bool packed(const BtArgs& a, bool backward) {
+  const int64_t ldo = (int64_t)a.heads * a.dk;
+  return !whole_rows(a, a.q, a.ldq, a.bq) || !whole_rows(a, a.k, a.ldk, a.bk) || !whole_rows(a, a.v, a.ldv, a.bv) ||
+         (backward && !whole_rows(a, a.dout, ldo, ldo));
+}
+int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+// bytes of packed q (and dout) and of packed k (and v)
+struct Packed { int64_t q, k; };
+Packed packed_space(const BtArgs& a) {
+  const int64_t per = 16 / (int64_t)esize(a), row = (a.dk + per - 1) / per * 16;
+  return {up((int64_t)a.n * a.lq * a.heads * row), up((int64_t)a.n * a.lk * a.kv_heads * row)};
 }
 
 // Few rows: the rows of a kv head's query heads fill one MFMA tile (32), or the tiled kernel's blocks of 128
@@ -67,13 +81,16 @@ int dkv_splits(const BtArgs& a) {
 }
 int dk_class(const BtArgs& a) { return a.dk <= 32 ? 32 : a.dk <= 64 ? 64 : 128; }
 
-int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-
-// the backward workspace: delta, the blocks' table gradients (bf16: two lists, and BtArgs::rest), then the parts of dq and
+// the backward workspace: packed rows, delta, the blocks' table gradients (bf16: two lists, and BtArgs::rest), then the parts of dq and
 // later of dk and dv
-struct Space { int64_t delta, table, rest, part; };
+struct Space {
+  int64_t pack, delta, table, rest, part;
+  int64_t all() const { return pack + delta + table + rest + part; }
+};
 Space backward_space(const BtArgs& a) {
   Space s;
+  const Packed p = packed_space(a);
+  s.pack = packed(a, true) ? 2 * (p.q + p.k) : 0;
   s.delta = up((int64_t)a.n * a.heads * a.lq * 4);
   const int ds = dq_splits(a), ks = dkv_splits(a);
   const int two = a.dtype == GGD_TR_BF16;
@@ -84,15 +101,40 @@ Space backward_space(const BtArgs& a) {
   s.part = up(std::max(pq, pk));
   return s;
 }
-int64_t forward_space(const BtArgs& a) {
-  if (!few_rows(a)) return 0;
-  const int s = few_splits(a);
-  if (s == 1) return 0;
-  const int64_t rows = ((int64_t)a.group * a.lq + 31) / 32 * 32 * a.n * a.kv_heads;
-  return up(rows * s * (dk_class(a) + 4) * 4);
+Space forward_space(const BtArgs& a) {
+  Space s{};
+  const Packed p = packed_space(a);
+  if (packed(a, false)) s.pack = p.q + 2 * p.k;
+  if (few_rows(a) && few_splits(a) > 1)
+    s.part = up(((int64_t)a.group * a.lq + 31) / 32 * 32 * a.n * a.kv_heads * few_splits(a) * (dk_class(a) + 4) * 4);
+  return s;
 }
 
 const Launch& launch(const BtArgs& a) { return a.dtype == GGD_TR_F32 ? battn_f32(a) : pick<bf16_t>(a); }
+
+
+// q, k, v (and dout) as the kernels read them, packed into the workspace's first part where they have to be
+hipError_t rows(BtArgs& a, bool backward, hipStream_t s) {
+  a.hq = a.hk = a.dk;
+  a.lddo = (int64_t)a.heads * a.dk;
+  if (!packed(a, backward)) return hipSuccess;
+  const Packed p = packed_space(a);
+  const int64_t per = 16 / (int64_t)esize(a), dkp = (a.dk + per - 1) / per * per;
+  char* at = (char*)a.ws;
+  const Launch& l = launch(a);
+  if (const hipError_t e = l.pack(a, a.q, a.ldq, a.bq, a.lq, a.heads, at, s)) return e;
+  if (const hipError_t e = l.pack(a, a.k, a.ldk, a.bk, a.lk, a.kv_heads, at + p.q, s)) return e;
+  if (const hipError_t e = l.pack(a, a.v, a.ldv, a.bv, a.lk, a.kv_heads, at + p.q + p.k, s)) return e;
+  if (backward) {
+    if (const hipError_t e = l.pack(a, a.dout, a.lddo, a.lq * a.lddo, a.lq, a.heads, at + p.q + 2 * p.k, s)) return e;
+    a.dout = at + p.q + 2 * p.k;
+  }
+  a.q = at, a.k = at + p.q, a.v = at + p.q + p.k;
+  a.hq = a.hk = dkp;
+  a.ldq = a.lddo = a.heads * dkp, a.bq = a.lq * a.ldq;
+  a.ldk = a.ldv = a.kv_heads * dkp, a.bk = a.bv = a.lk * a.ldk;
+  return hipSuccess;
+}
 
 }  // namespace
 }  // namespace battn
@@ -106,9 +148,7 @@ extern "C" {
 int64_t ggd_tr_battn_ws(const ggd_tr_battn_args* args, int backward) {
   BtArgs a{};
   if (prepare(args, a) || a.n == 0) return 0;
-  if (!backward) return forward_space(a);
-  const Space s = backward_space(a);
-  return s.delta + s.table + s.rest + s.part;
+  return (backward ? backward_space(a) : forward_space(a)).all();
 }
 
 int ggd_tr_battn_fwd(const ggd_tr_battn_args* args, void* stream) {
@@ -116,17 +156,16 @@ int ggd_tr_battn_fwd(const ggd_tr_battn_args* args, void* stream) {
   if (const int e = prepare(args, a)) return e;
   if (a.n == 0) return 0;
   if (!a.q || !a.k || !a.v || !a.o || !a.stat != !a.o32) return -1;
-  const int64_t need = forward_space(a);
-  if (need && (!a.ws || !aligned(a.ws, 16) || a.ws_bytes < need)) return -1;
-  a.vec = vec_rows(a, a.q, a.ldq, a.bq) && vec_rows(a, a.k, a.ldk, a.bk) && vec_rows(a, a.v, a.ldv, a.bv);
-  a.vec_o = a.dk % 4 == 0 && a.ldo % 4 == 0 && a.bo % 4 == 0 && aligned(a.o, 4 * esize(a)) && aligned(a.o32, 16);
+  const Space space = forward_space(a);
+  if (space.all() && (!a.ws || !aligned(a.ws, 16) || a.ws_bytes < space.all())) return -1;
   if (!aligned(a.stat, 8)) return -1;
-  if (few_rows(a)) {
-    a.splits = few_splits(a);
-    a.part = (float*)a.ws;
-    return launch(a).few(a, (hipStream_t)stream) == hipSuccess ? 0 : -3;
-  }
-  return launch(a).fwd(a, (hipStream_t)stream) == hipSuccess ? 0 : -3;
+  a.vec_o = a.dk % 4 == 0 && a.ldo % 4 == 0 && a.bo % 4 == 0 && aligned(a.o, 4 * esize(a)) && aligned(a.o32, 16);
+  const bool few = few_rows(a);
+  a.splits = few ? few_splits(a) : 1;
+  a.part = (float*)((char*)a.ws + space.pack);
+  const hipStream_t s = (hipStream_t)stream;
+  if (rows(a, false, s) != hipSuccess) return -3;
+  return (few ? launch(a).few(a, s) : launch(a).fwd(a, s)) == hipSuccess ? 0 : -3;
 }
 
 int ggd_tr_battn_bwd(const ggd_tr_battn_args* args, void* stream) {
@@ -134,19 +173,21 @@ int ggd_tr_battn_bwd(const ggd_tr_battn_args* args, void* stream) {
   if (const int e = prepare(args, a)) return e;
   if (a.n == 0) return 0;
   if (!a.q || !a.k || !a.v || !a.stat || !a.o32 || !a.dout || !a.dq || !a.dk_out || !a.dv || (a.dtable && !a.table)) return -1;
-  const Space s = backward_space(a);
-  if (!a.ws || !aligned(a.ws, 16) || a.ws_bytes < s.delta + s.table + s.rest + s.part || !aligned(a.stat, 8)) return -1;
-  a.delta = (float*)a.ws;
-  a.dtab = (float*)((char*)a.ws + s.delta);
-  a.rest = (float*)((char*)a.ws + s.delta + s.table);
-  a.part = (float*)((char*)a.ws + s.delta + s.table + s.rest);
-  const int64_t ldo = (int64_t)a.heads * a.dk;
-  a.vec = vec_rows(a, a.q, a.ldq, a.bq) && vec_rows(a, a.k, a.ldk, a.bk) && vec_rows(a, a.v, a.ldv, a.bv) && vec_rows(a, a.dout, ldo, ldo);
+  const Space space = backward_space(a);
+  if (!a.ws || !aligned(a.ws, 16) || a.ws_bytes < space.all() || !aligned(a.stat, 8) || !aligned(a.o32, a.dk % 4 ? 4 : 16)) return -1;
+  char* at = (char*)a.ws + space.pack;
+  a.delta = (float*)at;
+  a.dtab = (float*)(at + space.delta);
+  a.rest = (float*)(at + space.delta + space.table);
+  a.part = (float*)(at + space.delta + space.table + space.rest);
   a.vec_o = a.dk % 4 == 0 && aligned(a.dq, 4 * esize(a)) && aligned(a.dk_out, 4 * esize(a)) && aligned(a.dv, 4 * esize(a));
-  a.splits = dq_splits(a);
-  if (launch(a).dq(a, (hipStream_t)stream) != hipSuccess) return -3;
-  a.splits = dkv_splits(a);
-  return launch(a).dkv(a, (hipStream_t)stream) == hipSuccess ? 0 : -3;
+  const int dqs = dq_splits(a), dkvs = dkv_splits(a);
+  const hipStream_t s = (hipStream_t)stream;
+  if (rows(a, true, s) != hipSuccess) return -3;
+  a.splits = dqs;
+  if (launch(a).dq(a, s) != hipSuccess) return -3;
+  a.splits = dkvs;
+  return launch(a).dkv(a, s) == hipSuccess ? 0 : -3;
 }
 
 }  // extern "C"

@@ -105,35 +105,36 @@ __global__ void __launch_bounds__(256) bt_fwd_kernel(BtArgs a) {
   if constexpr (BIAS) bias_line(line, a, head);
   const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
   Frag<T, DK> q;
-  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.dk, a.dk, a.vec, there);
-  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.dk;
-  const T* vb = (const T*)a.v + clip * a.bv + (int64_t)(head / a.group) * a.dk;
+  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.hq, a.dk, there);
+  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.hk;
+  const T* vb = (const T*)a.v + clip * a.bv + (int64_t)(head / a.group) * a.hk;
   const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
   Softmax<DK> sm;
   sm.start();
-  Stage<T, DK, KT, 256> ks, vs;
-  uint64_t next = __ballot(mask_byte(mask, 0, KT, a.lk));
-  ks.load(kb, a.ldk, next, a.dk, a.vec, tid);
-  vs.load(vb, a.ldv, next, a.dk, a.vec, tid);
+  Tile<T, DK, KT> ks, vs;
+  ks.start(a.ldk, a.dk);
+  vs.start(a.ldv, a.dk);
+  uint64_t bits = __ballot(mask_byte(mask, 0, KT, a.lk));
+  ks.load(kb, a.ldk, bits, lds);
+  vs.load(vb, a.ldv, bits, lds + IMG);
   int nb = mask_byte(mask, KT, KT, a.lk);
   const int nt = (a.lk + KT - 1) / KT;
   for (int t = 0; t < nt; ++t) {
-    uint4 *kimg = lds + (t & 1) * 2 * IMG, *vimg = kimg + IMG;
-    ks.store(kimg, tid);
-    vs.store(vimg, tid);
-    const uint64_t bits = next;
-    next = __ballot(nb);
+    const uint4 *kimg = lds + (t & 1) * 2 * IMG, *vimg = kimg + IMG, *to = lds + (~t & 1) * 2 * IMG;
+    tile_ready();
+    const uint64_t next = __ballot(nb);
     kb += KT * a.ldk;
     vb += KT * a.ldv;
-    ks.load(kb, a.ldk, next, a.dk, a.vec, tid);
-    vs.load(vb, a.ldv, next, a.dk, a.vec, tid);
+    if (t + 1 < nt) {   // (no load may be under way when the block ends)
+      ks.load(kb, a.ldk, next, to);
+      vs.load(vb, a.ldv, next, to + IMG);
+    }
     nb = mask_byte(mask, (t + 2) * KT, KT, a.lk);
-    // a wave past this barrier has read the other buffer's tile before it: one barrier a tile
-    __syncthreads();
     if (bits && row0 < a.lq) {
       const int first = t * KT - a.off;
       attend<T, DK, BIAS, KT / 32>(sm, kimg, vimg, q, bits, a, line, first + 4 * h - i, first - (row0 + 31), first + 31 - row0);
     }
+    bits = next;
   }
   sm.template finish<T>();
   const bool some = there && sm.lr != 0.f;
@@ -185,11 +186,11 @@ __global__ void __launch_bounds__(256) bt_few_kernel(BtArgs a) {
   const int r = tile * 32 + (lane & 31), g = min(r, rows - 1) / a.lq, i = min(r, rows - 1) - g * a.lq, head = kvh * a.group + g;
   const bool there = r < rows && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
   Frag<T, DK> q;
-  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.dk, a.dk, a.vec, there);
+  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.hq, a.dk, there);
   const int per = (kt + a.splits - 1) / a.splits, end = min(kt, (split + 1) * per);
   int t = split * per + wave;
-  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)kvh * a.dk;
-  const T* vb = (const T*)a.v + clip * a.bv + (int64_t)kvh * a.dk;
+  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)kvh * a.hk;
+  const T* vb = (const T*)a.v + clip * a.bv + (int64_t)kvh * a.hk;
   const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
   uint4 *kimg = lds + wave * 2 * IMG, *vimg = kimg + IMG;
   Softmax<DK> sm;
@@ -197,8 +198,8 @@ __global__ void __launch_bounds__(256) bt_few_kernel(BtArgs a) {
   Stage<T, DK, 32, 64> ks, vs;
   auto bytes = [&](int tt) { return tt < end ? mask_byte(mask, tt * 32, 32, a.lk) : 0; };
   uint64_t next = __ballot(bytes(t));
-  ks.load(kb + (int64_t)t * 32 * a.ldk, a.ldk, next, a.dk, a.vec, lane);
-  vs.load(vb + (int64_t)t * 32 * a.ldv, a.ldv, next, a.dk, a.vec, lane);
+  ks.load(kb + (int64_t)t * 32 * a.ldk, a.ldk, next, a.dk, lane);
+  vs.load(vb + (int64_t)t * 32 * a.ldv, a.ldv, next, a.dk, lane);
   int nb = bytes(t + 4);
   for (; t < end; t += 4) {
     ks.store(kimg, lane);
@@ -206,8 +207,8 @@ __global__ void __launch_bounds__(256) bt_few_kernel(BtArgs a) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the image is the wave's own: its LDS operations run in order
     const uint64_t bits = next;
     next = __ballot(nb);
-    ks.load(kb + (int64_t)(t + 4) * 32 * a.ldk, a.ldk, next, a.dk, a.vec, lane);
-    vs.load(vb + (int64_t)(t + 4) * 32 * a.ldv, a.ldv, next, a.dk, a.vec, lane);
+    ks.load(kb + (int64_t)(t + 4) * 32 * a.ldk, a.ldk, next, a.dk, lane);
+    vs.load(vb + (int64_t)(t + 4) * 32 * a.ldv, a.ldv, next, a.dk, lane);
     nb = bytes(t + 8);
     if (bits) {
       f32x16 s = zero16();
@@ -387,8 +388,8 @@ __global__ void __launch_bounds__(256) bt_dq_kernel(BtArgs a) {
   const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
   const int64_t crow = ((clip * a.lq + i) * a.heads + head) * a.dk;   // of the contiguous rows
   Frag<T, DK> q, dO;
-  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.dk, a.dk, a.vec, there);
-  dO.load((const T*)a.dout + crow, a.dk, a.vec, there);
+  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.hq, a.dk, there);
+  dO.load((const T*)a.dout + (clip * a.lq + i) * a.lddo + (int64_t)head * a.hq, a.dk, there);
   float m = INFINITY, rl = 0.f, delta = 0.f;
   if (there) {
     const float2 st = *(const float2*)(a.stat + 2 * (ch * a.lq + i));
@@ -396,49 +397,60 @@ __global__ void __launch_bounds__(256) bt_dq_kernel(BtArgs a) {
     rl = st.y;
 #pragma unroll
     for (int s = 0; s < Frag<T, DK>::N; ++s) {
-      const int c = (2 * s + h) * EPU;
+      const uint32_t u[4] = {dO.x[s].x, dO.x[s].y, dO.x[s].z, dO.x[s].w};
 #pragma unroll
-      for (int e = 0; e < EPU; ++e)
-        if (c + e < a.dk) {
-          float x;
-          if constexpr (sizeof(T) == 4) x = __uint_as_float(e == 0 ? dO.x[s].x : e == 1 ? dO.x[s].y : e == 2 ? dO.x[s].z : dO.x[s].w);
-          else {
-            const uint32_t u = e < 2 ? dO.x[s].x : e < 4 ? dO.x[s].y : e < 6 ? dO.x[s].z : dO.x[s].w;
-            x = __uint_as_float(e & 1 ? u & 0xFFFF0000u : u << 16);
-          }
-          delta = fmaf(x, a.o32[crow + c + e], delta);
+      for (int f = 0; f < EPU; f += 4) {
+        const int c = (2 * s + h) * EPU + f;
+        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (a.dk % 4 == 0) {
+          if (c < a.dk) o = *(const f32x4*)(a.o32 + crow + c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < a.dk) o[e] = a.o32[crow + c + e];
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x = sizeof(T) == 4 ? u[e] : e & 1 ? u[(f + e) >> 1] & 0xFFFF0000u : u[(f + e) >> 1] << 16;
+          delta = fmaf(__uint_as_float(x), o[e], delta);
+        }
+      }
     }
   }
   delta = both_sum(delta);
   if (rl == 0.f) delta = 0.f;   // a row without a key: whatever its do
   if (split == 0 && h == 0 && i < a.lq) a.delta[ch * a.lq + i] = delta;
   const int kt = (a.lk + KT - 1) / KT, per = (kt + a.splits - 1) / a.splits, t0 = split * per, t1 = min(kt, t0 + per);
-  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.dk + (int64_t)t0 * KT * a.ldk;
-  const T* vb = (const T*)a.v + clip * a.bv + (int64_t)(head / a.group) * a.dk + (int64_t)t0 * KT * a.ldv;
+  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.hk + (int64_t)t0 * KT * a.ldk;
+  const T* vb = (const T*)a.v + clip * a.bv + (int64_t)(head / a.group) * a.hk + (int64_t)t0 * KT * a.ldv;
   const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
   f32x16 acc[DK / 32];
 #pragma unroll
   for (int mb = 0; mb < DK / 32; ++mb) acc[mb] = zero16();
   float past = 0.f, behind = 0.f;   // sums of ds at distances >= D, <= -D
   float rest = 0.f, w_past = 0.f;   // (before 1 / l) sums of ds, and of weights at distances >= D
-  Stage<T, DK, KT, 256> ks, vs;
+  Tile<T, DK, KT> ks, vs;
+  ks.start(a.ldk, a.dk);
+  vs.start(a.ldv, a.dk);
   uint64_t next = __ballot(t0 < t1 ? mask_byte(mask, t0 * KT, KT, a.lk) : 0);
-  ks.load(kb, a.ldk, next, a.dk, a.vec, tid);
-  vs.load(vb, a.ldv, next, a.dk, a.vec, tid);
+  if (t0 < t1) {
+    ks.load(kb, a.ldk, next, lds);
+    vs.load(vb, a.ldv, next, lds + IMG);
+  }
   int nb = t0 + 1 < t1 ? mask_byte(mask, (t0 + 1) * KT, KT, a.lk) : 0;
   for (int t = t0; t < t1; ++t) {
-    uint4 *kimg = lds + (t & 1) * 2 * IMG, *vimg = kimg + IMG;
-    ks.store(kimg, tid);
-    vs.store(vimg, tid);
+    const int buf = (t - t0) & 1;
+    const uint4 *kimg = lds + buf * 2 * IMG, *vimg = kimg + IMG, *to = lds + (buf ^ 1) * 2 * IMG;
+    tile_ready();
     const uint64_t bits = next;
     next = __ballot(nb);
     kb += KT * a.ldk;
     vb += KT * a.ldv;
-    ks.load(kb, a.ldk, next, a.dk, a.vec, tid);
-    vs.load(vb, a.ldv, next, a.dk, a.vec, tid);
+    if (t + 1 < t1) {
+      ks.load(kb, a.ldk, next, to);
+      vs.load(vb, a.ldv, next, to + IMG);
+    }
     nb = t + 2 < t1 ? mask_byte(mask, (t + 2) * KT, KT, a.lk) : 0;
-    __syncthreads();
     if (!bits || row0 >= a.lq) continue;
 #pragma unroll
     for (int b = 0; b < KT / 32; ++b) {
@@ -545,7 +557,7 @@ __global__ void __launch_bounds__(256) bt_table_rest_kernel(BtArgs a) {
   for (int d = tid; d < 4 * lines; d += 256) hist[d] = 0.f;
   const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
   Frag<T, DK> q;
-  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.dk, a.dk, a.vec, there);
+  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.hq, a.dk, there);
   float m = INFINITY, rl = 0.f, e = 0.f, past = 0.f, near = 0.f;
   if (there) {
     const float2 st = *(const float2*)(a.stat + 2 * (ch * a.lq + i));
@@ -559,21 +571,22 @@ __global__ void __launch_bounds__(256) bt_table_rest_kernel(BtArgs a) {
   // keys within the distance of one of the block's queries: j - i - off in -D + 1 .. D - 1
   const int64_t j0 = (int64_t)first + a.off - D + 1, j1 = (int64_t)min(first + BT_ROWS, a.lq) - 1 + a.off + D;
   const int t0 = (int)max((int64_t)0, min(j0, (int64_t)a.lk)) / KT, t1 = (int)((max((int64_t)0, min(j1, (int64_t)a.lk)) + KT - 1) / KT);
-  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.dk + (int64_t)t0 * KT * a.ldk;
+  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.hk + (int64_t)t0 * KT * a.ldk;
   const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
-  Stage<T, DK, KT, 256> ks;
+  Tile<T, DK, KT> ks;
+  ks.start(a.ldk, a.dk);
   uint64_t next = __ballot(t0 < t1 ? mask_byte(mask, t0 * KT, KT, a.lk) : 0);
-  ks.load(kb, a.ldk, next, a.dk, a.vec, tid);
+  if (t0 < t1) ks.load(kb, a.ldk, next, lds);
   int nb = t0 + 1 < t1 ? mask_byte(mask, (t0 + 1) * KT, KT, a.lk) : 0;
   for (int t = t0; t < t1; ++t) {
-    uint4* kimg = lds + (t & 1) * IMG;
-    ks.store(kimg, tid);
+    const int buf = (t - t0) & 1;
+    const uint4* kimg = lds + buf * IMG;
+    tile_ready();
     const uint64_t bits = next;
     next = __ballot(nb);
     kb += KT * a.ldk;
-    ks.load(kb, a.ldk, next, a.dk, a.vec, tid);
+    if (t + 1 < t1) ks.load(kb, a.ldk, next, lds + (buf ^ 1) * IMG);
     nb = t + 2 < t1 ? mask_byte(mask, (t + 2) * KT, KT, a.lk) : 0;
-    __syncthreads();
     if (!bits || row0 >= a.lq) continue;
 #pragma unroll
     for (int b = 0; b < KT / 32; ++b) {
@@ -639,21 +652,22 @@ __global__ void __launch_bounds__(256) bt_dkv_kernel(BtArgs a) {
   const bool there = j < a.lk && (!mask || mask[j]);
   const bool live = __ballot(there);
   Frag<T, DK> k, v;
-  k.load((const T*)a.k + clip * a.bk + (int64_t)j * a.ldk + (int64_t)kvh * a.dk, a.dk, a.vec, there);
-  v.load((const T*)a.v + clip * a.bv + (int64_t)j * a.ldv + (int64_t)kvh * a.dk, a.dk, a.vec, there);
+  k.load((const T*)a.k + clip * a.bk + (int64_t)j * a.ldk + (int64_t)kvh * a.hk, a.dk, there);
+  v.load((const T*)a.v + clip * a.bv + (int64_t)j * a.ldv + (int64_t)kvh * a.hk, a.dk, there);
   f32x16 dk[DK / 32], dv[DK / 32];
 #pragma unroll
   for (int mb = 0; mb < DK / 32; ++mb) dk[mb] = dv[mb] = zero16();
   const int qt = (a.lq + QT - 1) / QT, steps = a.group * qt, per = (steps + a.splits - 1) / a.splits;
   const int s0 = any ? split * per : 0, s1 = any ? min(steps, s0 + per) : 0;
   const uint8_t* q_mask = a.q_mask ? a.q_mask + clip * a.bq_mask : nullptr;
-  const int64_t ldo = (int64_t)a.heads * a.dk;
-  Stage<T, DK, QT, 256> qs, os;
+  Tile<T, DK, QT> qs, os;
+  qs.start(a.ldq, a.dk);
+  os.start(a.lddo, a.dk);
   float st_m = 0.f, st_r = 0.f, st_d = 0.f;
-  auto load = [&](int step, uint64_t bits) {
+  auto load = [&](int step, uint64_t bits, const uint4* img) {
     const int head = kvh * a.group + step / qt, i0 = step % qt * QT;
-    qs.load((const T*)a.q + clip * a.bq + (int64_t)i0 * a.ldq + (int64_t)head * a.dk, a.ldq, bits, a.dk, a.vec, tid);
-    os.load((const T*)a.dout + (clip * a.lq + i0) * ldo + (int64_t)head * a.dk, ldo, bits, a.dk, a.vec, tid);
+    qs.load((const T*)a.q + clip * a.bq + (int64_t)i0 * a.ldq + (int64_t)head * a.hq, a.ldq, bits, img);
+    os.load((const T*)a.dout + (clip * a.lq + i0) * a.lddo + (int64_t)head * a.hq, a.lddo, bits, img + IMG);
     if (tid < QT) {
       const int64_t at = (clip * a.heads + head) * a.lq + i0 + tid;
       const bool row = (bits >> tid) & 1;
@@ -662,25 +676,24 @@ __global__ void __launch_bounds__(256) bt_dkv_kernel(BtArgs a) {
       st_d = row ? a.delta[at] : 0.f;
     }
   };
-  auto bytes = [&](int step) { return step < s1 ? mask_byte(q_mask, step % qt * QT, QT, a.lq) : 0; };
-  uint64_t next = __ballot(bytes(s0));
-  if (s0 < s1) load(s0, next);
-  int nb = bytes(s0 + 1), lined = -1;
-  for (int t = s0; t < s1; ++t) {
-    const int buf = (t - s0) & 1;
-    uint4 *qimg = lds + buf * 2 * IMG, *oimg = qimg + IMG;
-    float* sts = stats + buf * 3 * QT;
-    qs.store(qimg, tid);
-    os.store(oimg, tid);
+  auto put = [&](float* sts) {
     if (tid < QT) {
       sts[tid] = st_m;
       sts[QT + tid] = st_r;
       sts[2 * QT + tid] = st_d;
     }
-    const uint64_t bits = next;
-    next = __ballot(nb);
-    if (t + 1 < s1) load(t + 1, next);
-    nb = bytes(t + 2);
+  };
+  auto bytes = [&](int step) { return step < s1 ? mask_byte(q_mask, step % qt * QT, QT, a.lq) : 0; };
+  uint64_t next = __ballot(bytes(s0));
+  if (s0 < s1) {
+    load(s0, next, lds);
+    put(stats);
+  }
+  int nb = bytes(s0 + 1), lined = -1;
+  for (int t = s0; t < s1; ++t) {
+    const int buf = (t - s0) & 1;
+    const uint4 *qimg = lds + buf * 2 * IMG, *oimg = qimg + IMG;
+    const float* sts = stats + buf * 3 * QT;
     if constexpr (BIAS) {
       if (t / qt != lined) {   // another head: its line, once all have done with the last one's
         __syncthreads();
@@ -688,8 +701,12 @@ __global__ void __launch_bounds__(256) bt_dkv_kernel(BtArgs a) {
         bias_line(line, a, kvh * a.group + lined);
       }
     }
-    __syncthreads();
-    if (!bits || !live) continue;
+    tile_ready();
+    const uint64_t bits = next;
+    next = __ballot(nb);
+    if (t + 1 < s1) load(t + 1, next, lds + (buf ^ 1) * 2 * IMG);
+    nb = bytes(t + 2);
+    if (bits && live) {
 #pragma unroll
     for (int b = 0; b < QT / 32; ++b) {
       if (!(uint32_t)(bits >> (32 * b))) continue;
@@ -714,6 +731,8 @@ __global__ void __launch_bounds__(256) bt_dkv_kernel(BtArgs a) {
       mma_cols<T, DK>(dv, oimg, 32 * b, s);
       mma_cols<T, DK>(dk, qimg, 32 * b, dp);
     }
+    }
+    put(stats + (buf ^ 1) * 3 * QT);
   }
   if (j >= a.lk) return;
   if (!there)
@@ -726,6 +745,17 @@ __global__ void __launch_bounds__(256) bt_dkv_kernel(BtArgs a) {
   } else {
     store_row<float, DK>(a.part + split * all + row, dk, a.scale, a.dk, a.vec_o);
     store_row<float, DK>(a.part + (a.splits + split) * all + row, dv, 1.f, a.dk, a.vec_o);
+  }
+}
+
+// rows of heads that are not whole aligned 16-byte units, laid out anew as such: (clips rows heads) dkp elements, zeros past dk
+template <typename T>
+__global__ void __launch_bounds__(256) bt_pack_kernel(int64_t n, int rows, int heads, int dk, int dkp, const T* __restrict__ src, int64_t ld,
+                                                      int64_t b, T* __restrict__ dst) {
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
+    const int c = (int)(e % dkp);
+    const int64_t r = e / dkp / heads;
+    dst[e] = c < dk ? src[r / rows * b + r % rows * ld + (e / dkp % heads) * dk + c] : (T)0;
   }
 }
 
@@ -745,6 +775,16 @@ __global__ void __launch_bounds__(256) bt_sum_kernel(int64_t n, int splits, cons
 template <typename T>
 hipError_t sum_parts(int64_t n, int splits, const float* part, void* out, hipStream_t s) {
   hipLaunchKernelGGL(bt_sum_kernel<T>, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, s, n, splits, part, (T*)out);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t pack_rows(const BtArgs& a, const void* src, int64_t ld, int64_t b, int rows, int heads, void* dst, hipStream_t s) {
+  constexpr int per = 16 / sizeof(T);
+  const int dkp = (a.dk + per - 1) / per * per;
+  const int64_t n = (int64_t)a.n * rows * heads * dkp;
+  hipLaunchKernelGGL(bt_pack_kernel<T>, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 8192)), dim3(256), 0, s, n, rows, heads, a.dk, dkp,
+                     (const T*)src, ld, b, (T*)dst);
   return hipGetLastError();
 }
 
@@ -806,7 +846,7 @@ struct Kernels {
     if (const hipError_t e = sum_parts<T>(all, a.splits, a.part, a.dk_out, s)) return e;
     return sum_parts<T>(all, a.splits, a.part + a.splits * all, a.dv, s);
   }
-  static constexpr Launch launch = {fwd, few, dq, dkv};
+  static constexpr Launch launch = {pack_rows<T>, fwd, few, dq, dkv};
 };
 
 template <typename T>
