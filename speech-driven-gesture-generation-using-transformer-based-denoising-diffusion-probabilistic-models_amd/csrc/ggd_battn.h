@@ -233,6 +233,9 @@ __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DK / 32], const uint4* im
       }
     }
   } else {
+    if constexpr (SUM)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) *sum += p[r];
 #pragma unroll
     for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -311,11 +314,24 @@ __device__ __forceinline__ void bias_line(float* line, const BtArgs& a, int head
     line[d] = bias_entry(a.table[(int64_t)bucket_of(a, d) * a.heads + head]);
 }
 
+// a block of 32 x 32 places whose distances are lo .. hi: all past the table's distance?  They have one bias then.
+__device__ __forceinline__ bool past_table(int D, int lo, int hi) { return lo >= D || hi <= -D; }
+
+// ... and one that is worth adding behind the product's scale, in one fma with the maximum (not where it is so large that the
+// scores have to vanish beside it, or infinite)
+__device__ __forceinline__ bool one_bias(const float* line, int D, int lo, int hi, float& bias) {
+  if (!past_table(D, lo, hi)) return false;
+  const float b = line[lo >= D ? 2 * D : 0];
+  if (!(__builtin_amdgcn_readfirstlane(__float_as_int(fabsf(b))) < __float_as_int(4096.f))) return false;
+  bias = b;
+  return true;
+}
+
 // s (raw products) -> log2 units with the bias.  rel: j - i - offset of register row 0 of this half and this lane,
 // and sign +1 where the registers run over keys, -1 where they run over queries
 template <int SIGN>
 __device__ __forceinline__ void add_bias(f32x16& s, const float* line, float c, int rel, int D, int lo, int hi) {
-  if (lo >= D || hi <= -D) {   // the whole block is past the table's distance: one value
+  if (past_table(D, lo, hi)) {
     const float b = line[lo >= D ? 2 * D : 0];
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
@@ -324,6 +340,38 @@ __device__ __forceinline__ void add_bias(f32x16& s, const float* line, float c, 
     for (int r = 0; r < 16; ++r) {
       const int d = min(max(rel + SIGN * (8 * (r >> 2) + (r & 3)), -D), D) + D;
       s[r] = fmaf(s[r], c, line[d]);
+    }
+  }
+}
+
+// Sums over the diagonals (equal key - query) of a 32 x 32 block in registers, lane & 31 = query i, register row = key k, into a
+// histogram over clamped distances.  16 queries at a time go through an image of the wave's own, [k - i + 15][i], whose
+// rows lanes then read: all 32 lanes of the writes and all groups of 16 of the reads are in different banks.  Cells
+// without a place stay the zeros of diag_start.  Every lane adds another distance: one order, no two on one word.
+constexpr int DIAG = 48 * 20;   // floats of an image
+__device__ __forceinline__ void diag_start(float* img) {
+  for (int e = lane_id(); e < DIAG; e += 64) img[e] = 0.f;
+}
+// d0: key 0 - query 0 of the block (with the offset); hist: of distance 0; past, behind: sums at distances >= D, <= -D
+__device__ __forceinline__ void diag_add(float* img, float* hist, const f32x16& x, int d0, int D, float& past, float& behind) {
+  const int lane = lane_id(), h = lane >> 5, i = lane & 15;
+#pragma unroll
+  for (int ph = 0; ph < 2; ++ph) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (((lane >> 4) & 1) == ph) {
+      float* to = img + 80 * h + 300 - 19 * i;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) to[20 * (8 * (r >> 2) + (r & 3))] = x[r];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (lane < 47) {
+      const f32x4* row = (const f32x4*)(img + 20 * lane);
+      const f32x4 a = row[0] + row[1], b = row[2] + row[3], c = a + b;
+      const float sum = (c[0] + c[1]) + (c[2] + c[3]);
+      const int d = d0 - 16 * ph + lane - 15;
+      if (d >= D) past += sum;
+      else if (d <= -D) behind += sum;
+      else __hip_atomic_fetch_add(hist + d, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
     }
   }
 }

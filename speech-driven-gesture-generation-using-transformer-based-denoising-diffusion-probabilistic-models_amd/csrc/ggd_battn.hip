@@ -63,21 +63,30 @@ bool few_rows(const BtArgs& a) {
   return rows <= 32 || (blocks < 128 && a.lk >= 512 && a.lk >= 4 * a.lq);
 }
 
-// parts of a streamed axis of `tiles` tiles so that `blocks` blocks become about 512 (2 a CU), each with at least `least` tiles
-int parts(int64_t blocks, int64_t tiles, int64_t least) {
-  const int64_t want = (512 + blocks - 1) / std::max<int64_t>(1, blocks);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), tiles / least));
+// Parts of a streamed axis of `tiles` tiles: the fewest whose rounds of blocks over the chip's `slots` take (nearly) the least time,
+// each part with at least `least` tiles, at most 64 of them.
+int parts(int64_t blocks, int64_t tiles, int64_t least, int64_t slots) {
+  int best = 1;
+  double time = (double)((blocks + slots - 1) / slots);
+  for (int64_t s = 2; s <= std::min<int64_t>(64, tiles / least); ++s) {
+    const double t = (double)((blocks * s + slots - 1) / slots) / s;
+    if (t < 0.93 * time) best = (int)s, time = t;
+  }
+  return best;
 }
+// blocks that run at once: 256 CUs, and as many a CU as the kernel has waves a SIMD
+int64_t slots(const BtArgs& a, int bf16_dk, int f32_dk) { return a.dk <= (a.dtype == GGD_TR_BF16 ? bf16_dk : f32_dk) ? 512 : 256; }
 int few_splits(const BtArgs& a) {
   const int64_t blocks = (int64_t)a.n * a.kv_heads * (((int64_t)a.group * a.lq + 31) / 32);
-  return parts(blocks, (a.lk + 31) / 32, 8);
+  return parts(blocks, (a.lk + 31) / 32, 8, slots(a, 64, 32));
 }
 int tile(const BtArgs& a) { return a.dtype == GGD_TR_F32 && a.dk > 64 ? 32 : 64; }
 int dq_splits(const BtArgs& a) {
-  return parts((int64_t)a.n * a.heads * ((a.lq + BT_ROWS - 1) / BT_ROWS), (a.lk + tile(a) - 1) / tile(a), 4);
+  return parts((int64_t)a.n * a.heads * ((a.lq + BT_ROWS - 1) / BT_ROWS), (a.lk + tile(a) - 1) / tile(a), 4, slots(a, 128, 64));
 }
 int dkv_splits(const BtArgs& a) {
-  return parts((int64_t)a.n * a.kv_heads * ((a.lk + BT_ROWS - 1) / BT_ROWS), (int64_t)a.group * ((a.lq + tile(a) - 1) / tile(a)), 4);
+  return parts((int64_t)a.n * a.kv_heads * ((a.lk + BT_ROWS - 1) / BT_ROWS), (int64_t)a.group * ((a.lq + tile(a) - 1) / tile(a)), 4,
+               slots(a, 64, 32));
 }
 int dk_class(const BtArgs& a) { return a.dk <= 32 ? 32 : a.dk <= 64 ? 64 : 128; }
 

@@ -5,6 +5,8 @@
 namespace ggd {
 namespace battn {
 
+// Waves a SIMD in the kernels' launch bounds: 2 where the registers allow it (256 each).  The compiler then keeps the products'
+// results in VGPRs, where the VALU works on them; with 1 it gives the sums AGPRs, 256 more, and moves the scores.
 constexpr int BT_ROWS = 128;   // stationary rows of a block of the tiled kernels: 4 waves of 32
 
 // ---------------------------------------------------------------------------------------------
@@ -14,7 +16,7 @@ constexpr int BT_ROWS = 128;   // stationary rows of a block of the tiled kernel
 // ---------------------------------------------------------------------------------------------
 template <int DK>
 struct Softmax {
-  float m, l, lr;   // sums over this half's keys
+  float m, l, lr;   // sums over this half's keys (l: where it is kept, for the backward pass)
   f32x16 o[DK / 32];
   __device__ __forceinline__ void start() {
     m = -INFINITY;
@@ -25,8 +27,8 @@ struct Softmax {
   // this half's sums -> the row's; f32 rounds no weight, and has one sum
   template <typename T>
   __device__ __forceinline__ void finish() {
-    l = both_sum(l);
-    lr = sizeof(T) == 4 ? l : both_sum(lr);
+    lr = both_sum(lr);
+    l = sizeof(T) == 4 ? lr : both_sum(l);
   }
   __device__ __forceinline__ void raise(float mt) {   // mt: the blocks' maximum, the same in both halves
     if (__any(mt > m + 8.f)) {
@@ -57,30 +59,38 @@ __device__ __forceinline__ void attend(Softmax<DK>& sm, const uint4* kimg, const
                                        uint64_t bits, const BtArgs& a, const float* line, int rel, int lo, int hi) {
   const int h = lane_id() >> 5;
   f32x16 s[NB];
-  float mt = -INFINITY;
+  float mt = -INFINITY, f[NB], e[NB];   // scores in log2 units: f s + e
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     s[b] = zero16();
     mma_rows<T, DK>(s[b], kimg, 32 * b, q);
-    if constexpr (BIAS) add_bias<1>(s[b], line, a.c, rel + 32 * b, a.distance, lo + 32 * b, hi + 32 * b);
+    f[b] = a.c;
+    e[b] = 0.f;
+    if constexpr (BIAS) {
+      const int D = a.distance;
+      if (!one_bias(line, D, lo + 32 * b, hi + 32 * b, e[b])) {
+        add_bias<1>(s[b], line, a.c, rel + 32 * b, D, lo + 32 * b, hi + 32 * b);
+        f[b] = 1.f;
+      }
+    }
     const uint32_t w = (uint32_t)(bits >> (32 * b));
     if (w != 0xFFFFFFFFu) {
       const uint32_t w4 = w >> (4 * h);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[b][r] = row_bit(w4, r) ? s[b][r] : -INFINITY;
     }
-    mt = fmaxf(mt, max16(s[b]));
+    mt = fmaxf(mt, fmaf(max16(s[b]), f[b], e[b]));
   }
-  mt = both_max(mt);
-  if constexpr (!BIAS) mt *= a.c;
-  sm.raise(mt);
+  sm.raise(both_max(mt));
   const float m = sm.m == -INFINITY ? 0.f : sm.m;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
+    e[b] -= m;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[b][r] = __builtin_amdgcn_exp2f(BIAS ? s[b][r] - m : fmaf(s[b][r], a.c, -m));
-      sm.l += s[b][r];
+    for (int r = 0; r < 16; ++r) s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], f[b], e[b]));
+    if (sizeof(T) == 2 && a.stat) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sm.l += s[b][r];
     }
     mma_cols<T, DK, true>(sm.o, vimg, 32 * b, s[b], &sm.lr);
   }
@@ -90,7 +100,7 @@ __device__ __forceinline__ void attend(Softmax<DK>& sm, const uint4* kimg, const
 // forward, many rows: a block per 128 query rows of one head; the waves share the key tiles
 // ---------------------------------------------------------------------------------------------
 template <typename T, int DK, bool BIAS>
-__global__ void __launch_bounds__(256) bt_fwd_kernel(BtArgs a) {
+__global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) bt_fwd_kernel(BtArgs a) {
   constexpr int KT = tile_rows<T, DK>(), IMG = KT * Img<T, DK>::UPR;
   extern __shared__ uint4 lds[];
   float* line = (float*)(lds + 4 * IMG);
@@ -173,7 +183,7 @@ __device__ __forceinline__ void few_emit(const BtArgs& a, int64_t clip, int head
 }
 
 template <typename T, int DK, bool BIAS>
-__global__ void __launch_bounds__(256) bt_few_kernel(BtArgs a) {
+__global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1) bt_few_kernel(BtArgs a) {
   constexpr int IMG = 32 * Img<T, DK>::UPR, NU = DK / 4;
   extern __shared__ uint4 lds[];
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = tid >> 6;
@@ -239,7 +249,7 @@ __global__ void __launch_bounds__(256) bt_few_kernel(BtArgs a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[e] = __builtin_amdgcn_exp2f(BIAS ? s[e] - m : fmaf(s[e], a.c, -m));
-        sm.l += s[e];
+        if constexpr (sizeof(T) == 2) sm.l += s[e];
       }
       mma_cols<T, DK, true>(sm.o, vimg, 0, s, &sm.lr);
     }
@@ -331,9 +341,7 @@ __global__ void __launch_bounds__(256) bt_join_kernel(BtArgs a) {
 // ---------------------------------------------------------------------------------------------
 // dq (and delta, and the table's gradient): like the forward kernel, a block per 128 query rows of a head.
 // Weights stay without their row's 1 / l until the end: it is one factor of the lane's row.
-//   Table: a lane's ds go into a histogram over clamped distances.  The lanes of a half are consecutive queries,
-// so that one register's distances differ in all lanes: each wave adds to its own LDS copy, one half after
-// the other, without two lanes on one word -- the sums have one order.  Places past the table's distance
+//   Table: ds go into a histogram over clamped distances, a copy a wave (diag_add); blocks past the table's distance
 // are summed in registers.
 // ---------------------------------------------------------------------------------------------
 // the block's histogram copies and its lanes' sums past the distance -> a row of dtab.  first: the block's first query
@@ -359,19 +367,22 @@ __device__ __forceinline__ void write_buckets(const BtArgs& a, float* hist, floa
     which[d] = bucket_of(a, d);
   }
   __syncthreads();
-  for (int b = tid; b < a.n_buckets; b += 256) {
+  for (int b = wave; b < a.n_buckets; b += 4) {
     float x = 0.f;
-    for (int d = d0; d <= d1; ++d) x += which[d] == b ? hist[d] : 0.f;
-    a.dtab[row * a.n_buckets + b] = x;
+    for (int d = d0 + lane; d <= d1; d += 64) x += which[d] == b ? hist[d] : 0.f;
+    x = group_sum<16>(x);
+    x += __shfl_xor(x, 16);
+    x = both_sum(x);
+    if (lane == 0) a.dtab[row * a.n_buckets + b] = x;
   }
 }
 
 template <typename T, int DK, bool BIAS>
-__global__ void __launch_bounds__(256) bt_dq_kernel(BtArgs a) {
+__global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) bt_dq_kernel(BtArgs a) {
   constexpr int KT = tile_rows<T, DK>(), IMG = KT * Img<T, DK>::UPR, EPU = Img<T, DK>::EPU;
   extern __shared__ uint4 lds[];
   const int lines = 2 * a.distance + 1;
-  float *line = (float*)(lds + 4 * IMG), *hist = line + lines;   // hist: [4][lines], with a table gradient
+  float *line = (float*)(lds + 4 * IMG), *hist = line + (lines + 3) / 4 * 4;   // with a table gradient: [4][lines], and the diagonals' images
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = tid >> 6;
   const int qt = (a.lq + BT_ROWS - 1) / BT_ROWS;
   const int64_t items = (int64_t)a.n * a.heads * a.splits * qt, w = work_item(items);
@@ -382,8 +393,10 @@ __global__ void __launch_bounds__(256) bt_dq_kernel(BtArgs a) {
   const bool table_grad = BIAS && a.dtable;
   if constexpr (BIAS) {
     bias_line(line, a, head);
-    if (table_grad)
+    if (table_grad) {
       for (int d = tid; d < 4 * lines; d += 256) hist[d] = 0.f;
+      diag_start(hist + 4 * lines + wave * DIAG);
+    }
   }
   const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
   const int64_t crow = ((clip * a.lq + i) * a.heads + head) * a.dk;   // of the contiguous rows
@@ -459,10 +472,18 @@ __global__ void __launch_bounds__(256) bt_dq_kernel(BtArgs a) {
       f32x16 s = zero16(), dp = zero16();
       mma_rows<T, DK>(s, kimg, 32 * b, q);
       mma_rows<T, DK>(dp, vimg, 32 * b, dO);
-      const int first = t * KT + 32 * b - a.off, rel = first + 4 * h - i, lo = first - (row0 + 31), hi = first + 31 - row0;
-      if constexpr (BIAS) add_bias<1>(s, line, a.c, rel, D, lo, hi);
+      const int first = t * KT + 32 * b - a.off, lo = first - (row0 + 31), hi = first + 31 - row0;
+      float f = a.c, e = -m;   // scores less the maximum, in log2 units: f s + e
+      if constexpr (BIAS) {
+        float bias = 0.f;
+        if (!one_bias(line, D, lo, hi, bias)) {
+          add_bias<1>(s, line, a.c, first + 4 * h - i, D, lo, hi);
+          f = 1.f;
+        }
+        e += bias;
+      }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] - m : fmaf(s[r], a.c, -m));
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], f, e));
       if (w32 != 0xFFFFFFFFu) {
         const uint32_t w4 = w32 >> (4 * h);
 #pragma unroll
@@ -475,7 +496,7 @@ __global__ void __launch_bounds__(256) bt_dq_kernel(BtArgs a) {
       for (int r = 0; r < 16; ++r) dp[r] = s[r] * (dp[r] - delta);
       if constexpr (BIAS) {
         if (table_grad) {
-          if (lo >= D || hi <= -D) {
+          if (past_table(D, lo, hi)) {
             float x = 0.f, y = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) x += dp[r];
@@ -489,22 +510,16 @@ __global__ void __launch_bounds__(256) bt_dq_kernel(BtArgs a) {
               behind = fmaf(x, rl, behind);
             }
           } else {
-            float* mine = hist + wave * lines + D;
+            f32x16 x;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int d = rel + 8 * (r >> 2) + (r & 3);
-              const float x = dp[r] * rl;
               rest += dp[r];
-              if (d >= D) {
-                past += x;
-                w_past += s[r];
-              } else if (d <= -D) {
-                behind += x;
-              } else if (h == 0) {
-                __hip_atomic_fetch_add(mine + d, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-              }
-              if (d < D && d > -D && h == 1) __hip_atomic_fetch_add(mine + d, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+              x[r] = dp[r] * rl;
             }
+            if (hi >= D)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) w_past += first + reg_row(r, h) - i >= D ? s[r] : 0.f;
+            diag_add(hist + 4 * lines + wave * DIAG, hist + wave * lines + D, x, first - row0, D, past, behind);
           }
         }
       }
@@ -541,11 +556,11 @@ __global__ void __launch_bounds__(256) bt_dq_kernel(BtArgs a) {
 // much: this kernel takes sum_i p_ij e_i off each distance's sum.  Only the places within the table's distance
 // are formed again (scores alone); the weights past it were summed on the way, and those behind are the remainder to 1.
 template <typename T, int DK>
-__global__ void __launch_bounds__(256) bt_table_rest_kernel(BtArgs a) {
+__global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
   constexpr int KT = tile_rows<T, DK>(), IMG = KT * Img<T, DK>::UPR;
   extern __shared__ uint4 lds[];
   const int lines = 2 * a.distance + 1, D = a.distance;
-  float *line = (float*)(lds + 2 * IMG), *hist = line + lines;
+  float *line = (float*)(lds + 2 * IMG), *hist = line + (lines + 3) / 4 * 4;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = tid >> 6;
   const int qt = (a.lq + BT_ROWS - 1) / BT_ROWS;
   const int64_t items = (int64_t)a.n * a.heads * qt, w = work_item(items);
@@ -555,6 +570,7 @@ __global__ void __launch_bounds__(256) bt_table_rest_kernel(BtArgs a) {
   const int head = (int)(ch % a.heads);
   bias_line(line, a, head);
   for (int d = tid; d < 4 * lines; d += 256) hist[d] = 0.f;
+  diag_start(hist + 4 * lines + wave * DIAG);
   const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
   Frag<T, DK> q;
   q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.hq, a.dk, there);
@@ -592,20 +608,20 @@ __global__ void __launch_bounds__(256) bt_table_rest_kernel(BtArgs a) {
     for (int b = 0; b < KT / 32; ++b) {
       const uint32_t w32 = (uint32_t)(bits >> (32 * b));
       const int at = t * KT + 32 * b - a.off, rel = at + 4 * h - i, lo = at - (row0 + 31), hi = at + 31 - row0;
-      if (!w32 || lo >= D || hi <= -D) continue;
+      if (!w32 || past_table(D, lo, hi)) continue;
       f32x16 s = zero16();
       mma_rows<T, DK>(s, kimg, 32 * b, q);
       add_bias<1>(s, line, a.c, rel, D, lo, hi);
       const uint32_t w4 = w32 >> (4 * h);
-      float* mine = hist + wave * lines + D;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int d = rel + 8 * (r >> 2) + (r & 3);
         const float p = rl != 0.f && row_bit(w4, r) && d < D && d > -D ? __builtin_amdgcn_exp2f(s[r] - m) * rl : 0.f;
         near += p;
-        if (d < D && d > -D && h == 0) __hip_atomic_fetch_add(mine + d, -e * p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-        if (d < D && d > -D && h == 1) __hip_atomic_fetch_add(mine + d, -e * p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        s[r] = -e * p;
       }
+      float none = 0.f;
+      diag_add(hist + 4 * lines + wave * DIAG, hist + wave * lines + D, s, at - row0, D, none, none);
     }
   }
   near = both_sum(near);
@@ -635,7 +651,7 @@ static __global__ void __launch_bounds__(64) bt_table_kernel(BtArgs a, int per, 
 // a shared head's gradient is one sum in registers
 // ---------------------------------------------------------------------------------------------
 template <typename T, int DK, bool BIAS>
-__global__ void __launch_bounds__(256) bt_dkv_kernel(BtArgs a) {
+__global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1) bt_dkv_kernel(BtArgs a) {
   constexpr int QT = tile_rows<T, DK>(), IMG = QT * Img<T, DK>::UPR;
   extern __shared__ uint4 lds[];
   // [2][q, do images], [2][3][QT] statistics (maximum, 1 / sum, delta), the bias line
@@ -794,6 +810,8 @@ struct Kernels {
   static constexpr size_t IMAGES = 4 * (size_t)KT * Img<T, DK>::UPR * 16;
   static size_t lines(const BtArgs& a) { return BIAS ? (2 * (size_t)a.distance + 1) * sizeof(float) : 0; }
 
+  static size_t table_lds(const BtArgs& a) { return 5 * lines(a) + 16 + 4 * DIAG * sizeof(float); }
+
   static hipError_t fwd(const BtArgs& a, hipStream_t s) {
     static std::atomic<bool> done[64];
     const size_t lds = IMAGES + lines(a);
@@ -815,7 +833,7 @@ struct Kernels {
   }
   static hipError_t dq(const BtArgs& a, hipStream_t s) {
     static std::atomic<bool> done[64];
-    const size_t lds = IMAGES + lines(a) * (a.dtable ? 5 : 1);
+    const size_t lds = IMAGES + (a.dtable ? table_lds(a) : lines(a));
     if (const hipError_t e = allow_lds(bt_dq_kernel<T, DK, BIAS>, lds, done)) return e;
     const int qt = (a.lq + BT_ROWS - 1) / BT_ROWS;
     hipLaunchKernelGGL((bt_dq_kernel<T, DK, BIAS>), dim3(work_grid((int64_t)a.n * a.heads * qt * a.splits)), dim3(256), lds, s, a);
@@ -824,7 +842,7 @@ struct Kernels {
       if (a.dtable) {
         if constexpr (sizeof(T) == 2) {
           static std::atomic<bool> rest_done[64];
-          const size_t rest_lds = IMAGES / 2 + lines(a) * 5;
+          const size_t rest_lds = IMAGES / 2 + table_lds(a);
           if (const hipError_t e = allow_lds(bt_table_rest_kernel<T, DK>, rest_lds, rest_done)) return e;
           hipLaunchKernelGGL((bt_table_rest_kernel<T, DK>), dim3(work_grid((int64_t)a.n * a.heads * qt)), dim3(256), rest_lds, s, a);
         }

@@ -126,10 +126,7 @@ def build(force=False, verbose=False):
     flags = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-fno-slp-vectorize", "-Xclang", "-target-feature",
              "-Xclang", "-packed-fp32-ops", "-Wno-unused-value", "-Wno-unused-result"]
     os.makedirs(os.path.join(PKG_DIR, "build"), exist_ok=True)
-    # the attention of any length reads every product's result on the VALU: with results in AGPRs each is moved first
-    # (8 moves for every exp2), and the kernels take more registers than two waves a SIMD have
-    vgpr_results = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-    units = [(src, src.replace(".hip", ".o"), vgpr_results if src.startswith("ggd_battn") else []) for src in SOURCES + DIAG_SOURCES]
+    units = [(src, src.replace(".hip", ".o"), []) for src in SOURCES + DIAG_SOURCES]
     units.append(("ggd_api.hip", "ggd_api_diag.o", ["-DGGD_DIAG"]))
     procs = []
     for src, obj_name, extra in units:  # one hipcc per translation unit, in parallel
