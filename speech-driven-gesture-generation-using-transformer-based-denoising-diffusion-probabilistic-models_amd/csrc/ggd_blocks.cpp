@@ -1,0 +1,337 @@
+// ggd_blocks.cpp -- the decoder-block operators' calls from Python (the _blocks module of blocks.py): argument checks, outputs and
+// workspaces from torch's allocator, and their nodes in torch's autograd graph, around the C entries of include/ggd_train.h.
+//
+// In C++ because a small call's time is the host's: with ctypes and torch.autograd.Function a training pass of cross attention
+// over 64 clips of 40 frames took 143 us of which its kernels are 34.  The entries come as addresses from native.py, so that
+// they are those of the library it loaded.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <optional>
+#include <sstream>
+#include <string>
+
+#include "../../include/ggd_train.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+struct Entries {
+  decltype(&ggd_tr_battn_fwd) battn_fwd;
+  decltype(&ggd_tr_battn_bwd) battn_bwd;
+  decltype(&ggd_tr_battn_ws) battn_ws;
+  decltype(&ggd_tr_resnorm_fwd) resnorm_fwd;
+  decltype(&ggd_tr_resnorm_bwd) resnorm_bwd;
+  decltype(&ggd_tr_resnorm_ws) resnorm_ws;
+} entries;
+
+// ValueError of what does not hold
+template <typename... A>
+[[noreturn]] void refuse(const char* what, const A&... parts) {
+  std::ostringstream s;
+  s << what << ": ";
+  (s << ... << parts);
+  throw py::value_error(s.str());
+}
+
+void check_status(int rc, const char* what) {
+  if (rc == -2) refuse(what, "unsupported shape");
+  TORCH_CHECK(rc == 0, what, " failed (ggd_train status ", rc, ")");
+}
+
+int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? GGD_TR_F32 : t.scalar_type() == at::kBFloat16 ? GGD_TR_BF16 : -1; }
+
+void on_gpu(const char* what, const Tensor& first) {
+  if (!first.is_cuda()) refuse(what, "the inputs have to be on a GPU device (no CPU fallback)");
+}
+void beside(const char* what, const char* name, const OptTensor& t, const Tensor& first) {
+  if (t && t->device() != first.device()) refuse(what, name, " has to be on ", first.device().str());
+}
+
+template <typename T = void>
+T* at_of(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
+Tensor or_none(const OptTensor& t) { return t ? *t : Tensor(); }
+OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+// the workspace of one call, which the allocator hands on in stream order
+Tensor workspace(int64_t bytes, const Tensor& like) { return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
+
+void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+// Gradients come once: where a graph of them is asked for, one that raises when it is used.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list real;
+  for (Tensor& g : grads)
+    if (g.defined()) real.push_back(g.detach().requires_grad_());
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", (int64_t)real.size());
+  real = (*error)(std::move(real));
+  size_t at = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = real[at++];
+  return grads;
+}
+
+// ------------------------------------------------------------------------------------------
+// attention
+// ------------------------------------------------------------------------------------------
+struct Inputs {
+  Tensor q, k, v, table, mask, q_mask, buckets;
+  int64_t heads, kv_heads, offset;
+  double scale;
+};
+
+ggd_tr_battn_args args_of(const Inputs& in) {
+  ggd_tr_battn_args a{};
+  const int64_t lq = in.q.size(1), width = in.q.size(2);
+  a.n = (int32_t)in.q.size(0), a.heads = (int32_t)in.heads, a.kv_heads = (int32_t)in.kv_heads, a.lq = (int32_t)lq, a.lk = (int32_t)in.k.size(1);
+  a.dk = (int32_t)(width / in.heads), a.dtype = dtype_of(in.q), a.scale = (float)in.scale;
+  a.q = in.q.data_ptr(), a.k = in.k.data_ptr(), a.v = in.v.data_ptr();
+  a.ldq = in.q.stride(1), a.bq = in.q.stride(0), a.ldk = in.k.stride(1), a.bk = in.k.stride(0), a.ldv = in.v.stride(1), a.bv = in.v.stride(0);
+  a.ldo = width, a.bo = lq * width;
+  if (in.mask.defined()) a.mask = at_of<const uint8_t>(in.mask), a.bmask = in.mask.stride(0);
+  if (in.q_mask.defined()) a.q_mask = at_of<const uint8_t>(in.q_mask), a.bq_mask = in.q_mask.stride(0);
+  if (in.table.defined()) {
+    a.table = at_of<const float>(in.table), a.buckets = at_of<const int32_t>(in.buckets);
+    a.n_buckets = (int32_t)in.table.size(0), a.distance = (int32_t)(in.buckets.size(0) / 2), a.offset = in.offset;
+  }
+  return a;
+}
+
+// o; with keep also what the backward pass needs (undefined where there is no query or no key: o is zeros then)
+Tensor attend(const Inputs& in, bool keep, Tensor& stat, Tensor& o32) {
+  Tensor o = at::empty({in.q.size(0), in.q.size(1), in.q.size(2)}, in.q.options());
+  if (o.numel() == 0 || in.k.size(1) == 0) return o.zero_();
+  const c10::DeviceGuard guard(in.q.device());
+  ggd_tr_battn_args a = args_of(in);
+  a.o = o.data_ptr();
+  if (keep) {
+    const auto f32 = in.q.options().dtype(at::kFloat);
+    stat = at::empty({in.q.size(0), in.heads, in.q.size(1), 2}, f32);
+    o32 = a.dtype == GGD_TR_F32 ? o : at::empty(o.sizes(), f32);
+    a.stat = at_of<float>(stat), a.o32 = at_of<float>(o32);
+  }
+  a.ws_bytes = entries.battn_ws(&a, 0);
+  const Tensor ws = workspace(a.ws_bytes, in.q);
+  a.ws = at_of(ws);
+  check_status(entries.battn_fwd(&a, stream_of(in.q)), "attention");
+  return o;
+}
+
+struct Attention : torch::autograd::Function<Attention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& table, const OptTensor& mask,
+                        const OptTensor& q_mask, const OptTensor& buckets, int64_t heads, int64_t kv_heads, double scale, int64_t offset) {
+    Tensor stat, o32;
+    const Inputs in{q, k, v, or_none(table), or_none(mask), or_none(q_mask), or_none(buckets), heads, kv_heads, offset, scale};
+    Tensor o = attend(in, true, stat, o32);
+    ctx->save_for_backward({q, k, v, in.table, in.mask, in.q_mask, in.buckets, stat, o32});
+    ctx->saved_data["heads"] = heads, ctx->saved_data["kv_heads"] = kv_heads, ctx->saved_data["scale"] = scale, ctx->saved_data["offset"] = offset;
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Inputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], ctx->saved_data["heads"].toInt(),
+                    ctx->saved_data["kv_heads"].toInt(), ctx->saved_data["offset"].toInt(), ctx->saved_data["scale"].toDouble()};
+    variable_list out(11);
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor &stat = saved[7], &o32 = saved[8];
+      for (int i = 0; i < 3; ++i) out[i] = at::empty(saved[i].sizes(), saved[i].options());
+      if (in.table.defined() && in.table.requires_grad()) out[3] = at::empty(in.table.sizes(), in.table.options());
+      if (!stat.defined()) {
+        for (Tensor& t : out)
+          if (t.defined()) t.zero_();
+      } else {
+        const c10::DeviceGuard guard(in.q.device());
+        const Tensor dout = grads[0].contiguous();
+        ggd_tr_battn_args a = args_of(in);
+        a.stat = at_of<float>(stat), a.o32 = at_of<float>(o32), a.dout = dout.data_ptr();
+        a.dq = out[0].data_ptr(), a.dk_out = out[1].data_ptr(), a.dv = out[2].data_ptr(), a.dtable = at_of<float>(out[3]);
+        a.ws_bytes = entries.battn_ws(&a, 1);
+        const Tensor ws = workspace(a.ws_bytes, in.q);
+        a.ws = at_of(ws);
+        const int rc = entries.battn_bwd(&a, stream_of(in.q));
+        TORCH_CHECK(rc == 0, "attention backward failed (ggd_train status ", rc, ")");
+      }
+    }
+    return once(std::move(out), "attention");
+  }
+};
+
+// (n, L, W) with contiguous rows: the tensor where its rows are, whatever their strides, else a copy
+Tensor rows(const Tensor& t) { return t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+Tensor mask_rows(const char* what, const char* name, const OptTensor& m, int64_t n, int64_t length) {
+  if (!m) return Tensor();
+  if (m->scalar_type() != at::kBool || m->dim() != 2 || m->size(0) != n || m->size(1) != length)
+    refuse(what, name, " has to be (", n, ", ", length, ") truth values");
+  return rows(*m);
+}
+
+Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tensor& v, int64_t heads, std::optional<int64_t> kv, std::optional<double> sc,
+                 const OptTensor& mask, const OptTensor& q_mask, const OptTensor& buckets, const OptTensor& table, int64_t offset) {
+  on_gpu(what, q);
+  beside(what, "k", k, q), beside(what, "v", v, q), beside(what, "mask", mask, q), beside(what, "q_mask", q_mask, q), beside(what, "table", table, q);
+  const int64_t kv_heads = kv.value_or(heads);
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads) refuse(what, heads, " heads over ", kv_heads, " kv heads");
+  if (q.dim() != 3 || k.dim() != 3 || v.dim() != 3) refuse(what, "q, k and v have to be (n, L, heads dk)");
+  const int64_t n = q.size(0), width = q.size(2), dk = width / heads;
+  if (width % heads || dk < 1 || dk > 128) refuse(what, "q rows of ", width, " elements are not ", heads, " heads of 1 to 128");
+  if (k.size(0) != n || k.size(2) != kv_heads * dk || v.sizes() != k.sizes())
+    refuse(what, "k ", k.sizes(), " and v ", v.sizes(), " have to be (", n, ", Lk, ", kv_heads * dk, ")");
+  if (dtype_of(q) < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
+    refuse(what, "q, k and v have to be of one type, float32 or bfloat16");
+  if (q.size(1) > 1 << 28 || k.size(1) > 1 << 28 || n > INT32_MAX || heads > INT32_MAX) refuse(what, "unsupported shape");
+  const double scale = sc.value_or(1.0 / std::sqrt((double)dk));
+  if (!(scale > 0.0 && scale <= 1e30)) refuse(what, "scale ", scale, " has to be positive");
+  Inputs in{rows(q), rows(k), rows(v), Tensor(), mask_rows(what, "mask", mask, n, k.size(1)), mask_rows(what, "q_mask", q_mask, n, q.size(1)),
+            or_none(buckets), heads, kv_heads, offset, scale};
+  if (table) in.table = table->contiguous();
+  const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (table && table->requires_grad()));
+  if (grad) return Attention::apply(in.q, in.k, in.v, given(in.table), given(in.mask), given(in.q_mask), given(in.buckets), heads, kv_heads, scale, offset);
+  Tensor stat, o32;
+  return attend(in, false, stat, o32);
+}
+
+// ------------------------------------------------------------------------------------------
+// the norms around a block
+// ------------------------------------------------------------------------------------------
+struct Shape {
+  int64_t rows, d, gate_rows, kind;
+  double scale, eps;
+};
+
+variable_list norm_forward(const Tensor& h, const Tensor& y, const Tensor& gate, const variable_list& w, const Shape& g, bool keep, Tensor& stats) {
+  Tensor h_out = at::empty_like(h), u = at::empty_like(h);
+  if (g.rows) {
+    const c10::DeviceGuard guard(h.device());
+    if (keep) stats = at::empty({4, g.rows}, h.options().dtype(at::kFloat));
+    check_status(entries.resnorm_fwd(g.rows, (int)g.d, dtype_of(h), (int)g.kind, (float)g.scale, (float)g.eps, at_of(h), at_of(y), at_of(gate), g.gate_rows,
+                                     at_of<float>(w[0]), at_of<float>(w[1]), at_of<float>(w[2]), at_of<float>(w[3]), at_of(h_out), at_of(u),
+                                     at_of<float>(stats), stream_of(h)),
+                 "residual_norm");
+  }
+  return {h_out, u};
+}
+
+struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& y, const OptTensor& gate, const OptTensor& post_g,
+                               const OptTensor& post_b, const OptTensor& pre_g, const OptTensor& pre_b, int64_t rows, int64_t d, int64_t gate_rows, int64_t kind, double scale, double eps) {
+    Tensor stats;
+    const variable_list w{or_none(post_g), or_none(post_b), or_none(pre_g), or_none(pre_b)};
+    variable_list out = norm_forward(h, y, or_none(gate), w, {rows, d, gate_rows, kind, scale, eps}, true, stats);
+    ctx->save_for_backward({h, y, or_none(gate), w[0], w[1], w[2], w[3], stats});
+    ctx->saved_data["rows"] = rows, ctx->saved_data["d"] = d, ctx->saved_data["gate_rows"] = gate_rows, ctx->saved_data["kind"] = kind;
+    ctx->saved_data["scale"] = scale, ctx->saved_data["eps"] = eps;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    auto whole = [&](const char* name) { return ctx->saved_data[name].toInt(); };
+    const int64_t rows = whole("rows"), d = whole("d"), gate_rows = whole("gate_rows"), kind = whole("kind");
+    const float scale = (float)ctx->saved_data["scale"].toDouble(), eps = (float)ctx->saved_data["eps"].toDouble();
+    variable_list out(13);
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor &h = saved[0], &y = saved[1], &gate = saved[2], &stats = saved[7];
+      for (int i = 0; i < 7; ++i)
+        if (saved[i].defined()) out[i] = at::empty_like(saved[i]);
+      if (rows == 0) {
+        for (Tensor& t : out)
+          if (t.defined()) t.zero_();
+      } else {
+        const c10::DeviceGuard guard(h.device());
+        const Tensor dh_out = grads[0].contiguous(), du = grads[1].contiguous();
+        const int64_t bytes = entries.resnorm_ws(rows, (int)d, gate_rows, gate.defined());
+        const Tensor ws = workspace(bytes, h);
+        const int rc = entries.resnorm_bwd(rows, (int)d, dtype_of(h), (int)kind, scale, eps, at_of(h), at_of(y), at_of(gate), gate_rows, at_of<float>(saved[3]),
+                                           at_of<float>(saved[4]), at_of<float>(saved[5]), at_of<float>(saved[6]), at_of<float>(stats), at_of(dh_out),
+                                           at_of(du), at_of(out[0]), at_of(out[1]), at_of(out[2]), at_of<float>(out[3]), at_of<float>(out[4]),
+                                           at_of<float>(out[5]), at_of<float>(out[6]), at_of(ws), bytes, stream_of(h));
+        TORCH_CHECK(rc == 0, "residual_norm backward failed (ggd_train status ", rc, ")");
+      }
+    }
+    return once(std::move(out), "residual_norm");
+  }
+};
+
+// Rows of h that share a row of the gate; the gate as it is read: leading dimensions of h, then ones, then d.  Any other shape
+// that broadcasts is expanded.
+int64_t gate_rows_of(const char* what, Tensor& gate, const Tensor& h) {
+  const int64_t dims = h.dim(), less = dims - gate.dim();
+  bool fits = gate.dim() >= 1 && less >= 0;
+  for (int64_t i = 0; fits && i < gate.dim(); ++i) fits = gate.size(i) == 1 || gate.size(i) == h.size(i + less);
+  if (!fits) refuse(what, "gate ", gate.sizes(), " does not broadcast to ", h.sizes());
+  auto size = [&](int64_t i) { return i < less ? 1 : gate.size(i - less); };
+  int64_t ones = dims - 1, shared = 1;
+  while (ones > 0 && size(ones - 1) == 1) --ones;
+  bool direct = size(dims - 1) == h.size(dims - 1);
+  for (int64_t i = 0; i < ones; ++i) direct = direct && size(i) == h.size(i);
+  if (!direct) {
+    gate = gate.expand(h.sizes()).contiguous();
+    return 1;
+  }
+  for (int64_t i = ones; i < dims - 1; ++i) shared *= h.size(i);
+  gate = gate.contiguous();
+  return std::max<int64_t>(1, shared);
+}
+
+std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre_g, const OptTensor& pre_b, const OptTensor& post_g, const OptTensor& post_b,
+                                        const OptTensor& gate_in, double scale, int64_t kind, double eps) {
+  const char* what = "residual_norm";
+  on_gpu(what, h);
+  if (!pre_g || (!post_g && post_b)) refuse(what, "a norm needs a weight");
+  beside(what, "y", y, h), beside(what, "gate", gate_in, h);
+  if (h.dim() < 1 || h.sizes() != y.sizes()) refuse(what, "h ", h.sizes(), " and y ", y.sizes(), " have to be of one shape");
+  if (dtype_of(h) < 0 || y.scalar_type() != h.scalar_type() || (gate_in && gate_in->scalar_type() != h.scalar_type()))
+    refuse(what, "h, y and gate have to be of one type, float32 or bfloat16");
+  const int64_t d = h.size(-1);
+  if (d < 1 || d > 8192) refuse(what, "rows of ", d, " elements: 1 to 8192");
+  variable_list w{or_none(post_g), or_none(post_b), or_none(pre_g), or_none(pre_b)};
+  bool grad = h.requires_grad() || y.requires_grad() || (gate_in && gate_in->requires_grad());
+  for (Tensor& t : w)
+    if (t.defined()) {
+      beside(what, "a weight or bias", t, h);
+      if (t.scalar_type() != at::kFloat || t.dim() != 1 || t.size(0) != d) refuse(what, "weights and biases have to be (", d, ",) in float32");
+      grad = grad || t.requires_grad();
+      t = t.contiguous();
+    }
+  if (!std::isfinite(scale) || !std::isfinite(eps) || !(eps > 0.0)) refuse(what, "scale ", scale, " has to be finite, eps ", eps, " positive");
+  Shape g{h.numel() / d, d, 1, kind, scale, eps};
+  Tensor gate = or_none(gate_in);
+  if (gate.defined()) g.gate_rows = gate_rows_of(what, gate, h);
+  h = h.contiguous(), y = y.contiguous();
+  variable_list out;
+  if (grad && at::GradMode::is_enabled()) {
+    out = ResidualNorm::apply(h, y, given(gate), given(w[0]), given(w[1]), given(w[2]), given(w[3]), g.rows, g.d, g.gate_rows, g.kind, g.scale, g.eps);
+  } else {
+    Tensor stats;
+    out = norm_forward(h, y, gate, w, g, false, stats);
+  }
+  return {out[0], out[1]};
+}
+
+void bind(const std::vector<uintptr_t>& at) {
+  if (at.size() != 6) throw py::value_error("six entries are wanted");
+  entries = {(decltype(entries.battn_fwd))at[0],   (decltype(entries.battn_bwd))at[1],   (decltype(entries.battn_ws))at[2],
+             (decltype(entries.resnorm_fwd))at[3], (decltype(entries.resnorm_bwd))at[4], (decltype(entries.resnorm_ws))at[5]};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_blocks, m) {
+  m.def("bind", &bind);
+  m.def("attention", &attention, py::call_guard<py::gil_scoped_release>());
+  m.def("residual_norm", &residual_norm, py::call_guard<py::gil_scoped_release>());
+}

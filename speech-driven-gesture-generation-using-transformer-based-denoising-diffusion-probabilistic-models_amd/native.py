@@ -16,12 +16,14 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 PRODUCT_LIB = os.path.join(PKG_DIR, "libggd.so")
 DIAG_LIB = os.path.join(PKG_DIR, "libggd_diag.so")
+BINDING = os.path.join(PKG_DIR, "_blocks.so")   # the decoder-block operators' calls (blocks.py), on torch's C++ side
 LIB_PATH = DIAG_LIB if os.environ.get("GGD_DIAG") == "1" else PRODUCT_LIB
 # A/B experiments (scripts/ab.sh): another build of the same library, same ABI
 if os.environ.get("GGD_LIB"):
     LIB_PATH = os.path.abspath(os.environ["GGD_LIB"])
 SOURCES = ["ggd_kernels.hip", "ggd_fused.hip", "ggd_mega.hip", "ggd_rows.hip", "ggd_persist.hip", "ggd_encoder.hip", "ggd_train.hip", "ggd_chain.hip", "ggd_attn.hip", "ggd_long.hip",
            "ggd_battn.hip", "ggd_battn_f32.hip", "ggd_resnorm.hip", "ggd_api.hip"]
+BINDING_SOURCE = "ggd_blocks.cpp"
 DIAG_SOURCES = ["ggd_diag.hip"]   # + ggd_api.hip again with -DGGD_DIAG
 HEADERS = ["ggd_kernels.h", "ggd_common.h", "ggd_chainlib.h", "ggd_fusedlib.h", "ggd_phases.h", "ggd_megasync.h", "ggd_battn.h", "ggd_battn_kernels.h",
            os.path.join("..", "..", "include", "ggd.h"),
@@ -109,7 +111,22 @@ def is_stale():
         t = os.path.getmtime(lib)
         if any(os.path.getmtime(p) > t for p in _sources()):
             return True
-    return False
+    return _binding_is_stale()
+
+
+def _binding_is_stale():
+    return not os.path.exists(BINDING) or any(os.path.getmtime(p) > os.path.getmtime(BINDING)
+                                              for p in _deps(os.path.join(CSRC, BINDING_SOURCE)))
+
+
+def _binding_command():
+    """g++ on the binding against torch's headers and libraries (which torch has loaded when it is)."""
+    import sysconfig
+    from torch.utils import cpp_extension
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"] +
+            ["-I" + d for d in cpp_extension.include_paths() + ["/opt/rocm/include", sysconfig.get_paths()["include"]]] +
+            [os.path.join(CSRC, BINDING_SOURCE), "-o", BINDING + ".tmp"] + ["-L" + d for d in cpp_extension.library_paths()] +
+            ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"])
 
 
 def build(force=False, verbose=False):
@@ -129,6 +146,12 @@ def build(force=False, verbose=False):
     units = [(src, src.replace(".hip", ".o"), []) for src in SOURCES + DIAG_SOURCES]
     units.append(("ggd_api.hip", "ggd_api_diag.o", ["-DGGD_DIAG"]))
     procs = []
+    binding = force or _binding_is_stale()
+    if binding:
+        cmd = _binding_command()
+        if verbose:
+            print(" ".join(cmd))
+        procs.append(subprocess.Popen(cmd, cwd=CSRC))
     for src, obj_name, extra in units:  # one hipcc per translation unit, in parallel
         obj = os.path.join(PKG_DIR, "build", obj_name)
         dep_t = max(os.path.getmtime(f) for f in _deps(os.path.join(CSRC, src)))
@@ -138,8 +161,10 @@ def build(force=False, verbose=False):
         if verbose:
             print(" ".join(cmd))
         procs.append(subprocess.Popen(cmd, cwd=CSRC))
-    if any(p.wait() != 0 for p in procs):
+    if any([p.wait() != 0 for p in procs]):
         raise RuntimeError("hipcc failed")
+    if binding:
+        os.replace(BINDING + ".tmp", BINDING)
     obj = lambda n: os.path.join(PKG_DIR, "build", n)
     product = [obj(s.replace(".hip", ".o")) for s in SOURCES]
     diag = [o for o in product if not o.endswith("ggd_api.o")] + [obj("ggd_api_diag.o"), obj("ggd_diag.o")]
@@ -240,6 +265,27 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_blocks = None
+
+
+def load_blocks():
+    """The decoder-block operators' binding, bound to the entries of the loaded library."""
+    global _blocks
+    if _blocks is None:
+        import importlib.machinery
+        import importlib.util
+        lib = load()
+        if not os.path.exists(BINDING):
+            raise ImportError(f"not built at {BINDING}; run __graft_entry__.build()")
+        loader = importlib.machinery.ExtensionFileLoader("_blocks", BINDING)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_blocks", BINDING, loader=loader))
+        loader.exec_module(module)
+        module.bind([ctypes.cast(getattr(lib, "ggd_tr_" + n), ctypes.c_void_p).value
+                     for n in ("battn_fwd", "battn_bwd", "battn_ws", "resnorm_fwd", "resnorm_bwd", "resnorm_ws")])
+        _blocks = module
+    return _blocks
 
 
 class GgdError(RuntimeError):
