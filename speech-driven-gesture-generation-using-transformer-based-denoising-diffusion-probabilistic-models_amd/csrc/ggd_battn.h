@@ -181,6 +181,14 @@ struct Frag {
 #pragma unroll
     for (int s = 0; s < N; ++s) x[s] = there ? load_unit(row, 2 * s + h, dk) : make_uint4(0, 0, 0, 0);
   }
+  // rows ld apart from `base` on, the same for the wave: zeros come from past the buffer's end, and no load waits for a branch
+  __device__ __forceinline__ void load_rows(const T* base, int64_t ld, int dk, bool there) {
+    const int l = lane_id(), h = l >> 5, row = (int)((l & 31) * ld * (int64_t)sizeof(T));
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), (short)0, 0x7FFFFFFF, 0x00020000);
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+      x[s] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, there && (2 * s + h) * Img<T, DK>::EPU < dk ? row + (2 * s + h) * 16 : BT_OUT, 0, 0));
+  }
 };
 
 // acc += rows r0 .. r0 + 31 of the image times the stationary rows (contraction over the elements)
@@ -298,7 +306,9 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, const f32x16 (&ac
 }
 
 // ---------------------------------------------------------------------------------------------
-// the bias: line[d + D] for d = clamp(j - i - offset, -D, D), in log2 units.  An entry of -inf forbids
+// the bias: line[d] of distance d = j - i - offset for -D - 62 .. D + 62, the ends' values past -D and D, in log2 units: a block of
+// 32 x 32 places that is not wholly past the table's distance finds each of its places there, and a lane's 16 at
+// constant steps from one address.  An entry of -inf forbids
 // its places; a finite one past the largest log2 unit counts as that, so that rows of the type's lowest
 // value stay a softmax among equals.
 // ---------------------------------------------------------------------------------------------
@@ -309,9 +319,14 @@ __device__ __forceinline__ float bias_entry(float x) {
 __device__ __forceinline__ int bucket_of(const BtArgs& a, int d) {   // d in 0 .. 2 D
   return min(max(a.buckets[d], 0), a.n_buckets - 1);
 }
-__device__ __forceinline__ void bias_line(float* line, const BtArgs& a, int head) {
-  for (int d = threadIdx.x; d <= 2 * a.distance; d += blockDim.x)
-    line[d] = bias_entry(a.table[(int64_t)bucket_of(a, d) * a.heads + head]);
+constexpr int LINE_PAD = 62;
+__device__ __host__ __forceinline__ int line_floats(int D) { return (2 * (D + LINE_PAD) + 1 + 3) / 4 * 4; }
+// mem: line_floats(D) floats; line = mem + D + LINE_PAD
+__device__ __forceinline__ void bias_line(float* mem, const BtArgs& a, int head) {
+  for (int e = threadIdx.x; e <= 2 * (a.distance + LINE_PAD); e += blockDim.x) {
+    const int d = min(max(e - LINE_PAD, 0), 2 * a.distance);
+    mem[e] = bias_entry(a.table[(int64_t)bucket_of(a, d) * a.heads + head]);
+  }
 }
 
 // a block of 32 x 32 places whose distances are lo .. hi: all past the table's distance?  They have one bias then.
@@ -321,7 +336,7 @@ __device__ __forceinline__ bool past_table(int D, int lo, int hi) { return lo >=
 // scores have to vanish beside it, or infinite)
 __device__ __forceinline__ bool one_bias(const float* line, int D, int lo, int hi, float& bias) {
   if (!past_table(D, lo, hi)) return false;
-  const float b = line[lo >= D ? 2 * D : 0];
+  const float b = line[lo >= D ? D : -D];
   if (!(__builtin_amdgcn_readfirstlane(__float_as_int(fabsf(b))) < __float_as_int(4096.f))) return false;
   bias = b;
   return true;
@@ -332,15 +347,13 @@ __device__ __forceinline__ bool one_bias(const float* line, int D, int lo, int h
 template <int SIGN>
 __device__ __forceinline__ void add_bias(f32x16& s, const float* line, float c, int rel, int D, int lo, int hi) {
   if (past_table(D, lo, hi)) {
-    const float b = line[lo >= D ? 2 * D : 0];
+    const float b = line[lo >= D ? D : -D];
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, b);
   } else {
+    const float* at = line + rel;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int d = min(max(rel + SIGN * (8 * (r >> 2) + (r & 3)), -D), D) + D;
-      s[r] = fmaf(s[r], c, line[d]);
-    }
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, at[SIGN * (8 * (r >> 2) + (r & 3))]);
   }
 }
 
@@ -378,10 +391,7 @@ __device__ __forceinline__ void diag_add(float* img, float* hist, const f32x16& 
 
 // XCD-aware block order: workgroups go to the 8 XCDs in turn; consecutive work items (the tiles that share
 // keys and values) go to one XCD, so that its L2 holds them once
-__device__ __forceinline__ int64_t work_item(int64_t items) {
-  const int64_t per = (items + 7) / 8;
-  return (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-}
+__device__ __forceinline__ uint32_t work_item(uint32_t items) { return (blockIdx.x & 7) * ((items + 7) / 8) + (blockIdx.x >> 3); }
 inline unsigned work_grid(int64_t items) { return (unsigned)((items + 7) / 8 * 8); }
 
 struct Launch {

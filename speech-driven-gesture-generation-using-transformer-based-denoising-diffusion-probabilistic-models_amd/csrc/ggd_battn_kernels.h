@@ -103,24 +103,16 @@ template <typename T, int DK, bool BIAS>
 __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) bt_fwd_kernel(BtArgs a) {
   constexpr int KT = tile_rows<T, DK>(), IMG = KT * Img<T, DK>::UPR;
   extern __shared__ uint4 lds[];
-  float* line = (float*)(lds + 4 * IMG);
-  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = tid >> 6;
-  const int qt = (a.lq + BT_ROWS - 1) / BT_ROWS;
-  const int64_t items = (int64_t)a.n * a.heads * qt, w = work_item(items);
+  float *mem = (float*)(lds + 4 * IMG), *line = mem + a.distance + LINE_PAD;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * qt, w = work_item(items);
   if (w >= items) return;
   const int row0 = (int)(w % qt) * BT_ROWS + wave * 32, i = row0 + (lane & 31);
-  const int64_t ch = w / qt;   // clip heads + head
-  const int head = (int)(ch % a.heads);
+  const int ch = w / qt, head = ch % a.heads;   // clip heads + head
   const int64_t clip = ch / a.heads;
-  if constexpr (BIAS) bias_line(line, a, head);
-  const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
-  Frag<T, DK> q;
-  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.hq, a.dk, there);
   const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.hk;
   const T* vb = (const T*)a.v + clip * a.bv + (int64_t)(head / a.group) * a.hk;
   const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
-  Softmax<DK> sm;
-  sm.start();
   Tile<T, DK, KT> ks, vs;
   ks.start(a.ldk, a.dk);
   vs.start(a.ldv, a.dk);
@@ -128,6 +120,12 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
   ks.load(kb, a.ldk, bits, lds);
   vs.load(vb, a.ldv, bits, lds + IMG);
   int nb = mask_byte(mask, KT, KT, a.lk);
+  const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
+  Frag<T, DK> q;
+  q.load_rows((const T*)a.q + clip * a.bq + (int64_t)row0 * a.ldq + (int64_t)head * a.hq, a.ldq, a.dk, there);
+  if constexpr (BIAS) bias_line(mem, a, head);
+  Softmax<DK> sm;
+  sm.start();
   const int nt = (a.lk + KT - 1) / KT;
   for (int t = 0; t < nt; ++t) {
     const uint4 *kimg = lds + (t & 1) * 2 * IMG, *vimg = kimg + IMG, *to = lds + (~t & 1) * 2 * IMG;
@@ -155,7 +153,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
     for (int mb = 0; mb < DK / 32; ++mb) sm.o[mb] = zero16();
   store_row<T, DK>((T*)a.o + clip * a.bo + (int64_t)i * a.ldo + (int64_t)head * a.dk, sm.o, inv, a.dk, a.vec_o);
   if (a.stat) {
-    if (h == 0) *(float2*)(a.stat + 2 * (ch * a.lq + i)) = make_float2(some ? sm.m : INFINITY, some ? 1.0f / sm.l : 0.f);
+    if (h == 0) *(float2*)(a.stat + 2 * ((int64_t)ch * a.lq + i)) = make_float2(some ? sm.m : INFINITY, some ? 1.0f / sm.l : 0.f);
     if (a.o32 != (float*)a.o)
       store_row<float, DK>(a.o32 + ((clip * a.lq + i) * a.heads + head) * a.dk, sm.o, inv, a.dk, a.vec_o);
   }
@@ -186,13 +184,12 @@ template <typename T, int DK, bool BIAS>
 __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1) bt_few_kernel(BtArgs a) {
   constexpr int IMG = 32 * Img<T, DK>::UPR, NU = DK / 4;
   extern __shared__ uint4 lds[];
-  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = a.group * a.lq, tiles = (rows + 31) / 32, kt = (a.lk + 31) / 32;
-  const int64_t items = (int64_t)a.n * a.kv_heads * a.splits * tiles, w = work_item(items);
+  const uint32_t items = a.n * a.kv_heads * a.splits * tiles, w = work_item(items);
   if (w >= items) return;
-  const int tile = (int)(w % tiles), split = (int)(w / tiles % a.splits);
-  const int64_t pair = w / tiles / a.splits, clip = pair / a.kv_heads;
-  const int kvh = (int)(pair % a.kv_heads);
+  const int tile = w % tiles, rest = w / tiles, split = rest % a.splits, pair = rest / a.splits, kvh = pair % a.kv_heads;
+  const int64_t clip = pair / a.kv_heads;
   const int r = tile * 32 + (lane & 31), g = min(r, rows - 1) / a.lq, i = min(r, rows - 1) - g * a.lq, head = kvh * a.group + g;
   const bool there = r < rows && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
   Frag<T, DK> q;
@@ -382,66 +379,17 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
   constexpr int KT = tile_rows<T, DK>(), IMG = KT * Img<T, DK>::UPR, EPU = Img<T, DK>::EPU;
   extern __shared__ uint4 lds[];
   const int lines = 2 * a.distance + 1;
-  float *line = (float*)(lds + 4 * IMG), *hist = line + (lines + 3) / 4 * 4;   // with a table gradient: [4][lines], and the diagonals' images
-  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = tid >> 6;
-  const int qt = (a.lq + BT_ROWS - 1) / BT_ROWS;
-  const int64_t items = (int64_t)a.n * a.heads * a.splits * qt, w = work_item(items);
+  float *mem = (float*)(lds + 4 * IMG), *line = mem + a.distance + LINE_PAD, *hist = mem + line_floats(a.distance);   // with a table gradient: [4][lines], and the diagonals' images
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * a.splits * qt, w = work_item(items);
   if (w >= items) return;
-  const int row0 = (int)(w % qt) * BT_ROWS + wave * 32, i = row0 + (lane & 31), split = (int)(w / qt % a.splits);
-  const int64_t ch = w / qt / a.splits, clip = ch / a.heads;
-  const int head = (int)(ch % a.heads), D = a.distance;
-  const bool table_grad = BIAS && a.dtable;
-  if constexpr (BIAS) {
-    bias_line(line, a, head);
-    if (table_grad) {
-      for (int d = tid; d < 4 * lines; d += 256) hist[d] = 0.f;
-      diag_start(hist + 4 * lines + wave * DIAG);
-    }
-  }
-  const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
-  const int64_t crow = ((clip * a.lq + i) * a.heads + head) * a.dk;   // of the contiguous rows
-  Frag<T, DK> q, dO;
-  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.hq, a.dk, there);
-  dO.load((const T*)a.dout + (clip * a.lq + i) * a.lddo + (int64_t)head * a.hq, a.dk, there);
-  float m = INFINITY, rl = 0.f, delta = 0.f;
-  if (there) {
-    const float2 st = *(const float2*)(a.stat + 2 * (ch * a.lq + i));
-    m = st.x;
-    rl = st.y;
-#pragma unroll
-    for (int s = 0; s < Frag<T, DK>::N; ++s) {
-      const uint32_t u[4] = {dO.x[s].x, dO.x[s].y, dO.x[s].z, dO.x[s].w};
-#pragma unroll
-      for (int f = 0; f < EPU; f += 4) {
-        const int c = (2 * s + h) * EPU + f;
-        f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (a.dk % 4 == 0) {
-          if (c < a.dk) o = *(const f32x4*)(a.o32 + crow + c);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < a.dk) o[e] = a.o32[crow + c + e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t x = sizeof(T) == 4 ? u[e] : e & 1 ? u[(f + e) >> 1] & 0xFFFF0000u : u[(f + e) >> 1] << 16;
-          delta = fmaf(__uint_as_float(x), o[e], delta);
-        }
-      }
-    }
-  }
-  delta = both_sum(delta);
-  if (rl == 0.f) delta = 0.f;   // a row without a key: whatever its do
-  if (split == 0 && h == 0 && i < a.lq) a.delta[ch * a.lq + i] = delta;
+  const int first_row = (int)(w % qt) * BT_ROWS, row0 = first_row + wave * 32, i = row0 + (lane & 31), split = w / qt % a.splits;
+  const int ch = w / qt / a.splits, head = ch % a.heads, D = a.distance;
+  const int64_t clip = ch / a.heads, srow = (int64_t)ch * a.lq + i;   // of the statistics
   const int kt = (a.lk + KT - 1) / KT, per = (kt + a.splits - 1) / a.splits, t0 = split * per, t1 = min(kt, t0 + per);
   const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.hk + (int64_t)t0 * KT * a.ldk;
   const T* vb = (const T*)a.v + clip * a.bv + (int64_t)(head / a.group) * a.hk + (int64_t)t0 * KT * a.ldv;
   const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
-  f32x16 acc[DK / 32];
-#pragma unroll
-  for (int mb = 0; mb < DK / 32; ++mb) acc[mb] = zero16();
-  float past = 0.f, behind = 0.f;   // sums of ds at distances >= D, <= -D
-  float rest = 0.f, w_past = 0.f;   // (before 1 / l) sums of ds, and of weights at distances >= D
   Tile<T, DK, KT> ks, vs;
   ks.start(a.ldk, a.dk);
   vs.start(a.ldv, a.dk);
@@ -451,6 +399,53 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
     vs.load(vb, a.ldv, next, lds + IMG);
   }
   int nb = t0 + 1 < t1 ? mask_byte(mask, (t0 + 1) * KT, KT, a.lk) : 0;
+  const bool mine = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
+  const float2 st = mine ? *(const float2*)(a.stat + 2 * srow) : make_float2(INFINITY, 0.f);
+  const float m = st.x, rl = st.y;
+  const bool there = rl != 0.f;   // a row that attends something: of another nothing is read, whatever its do
+  Frag<T, DK> q, dO;
+  q.load_rows((const T*)a.q + clip * a.bq + (int64_t)row0 * a.ldq + (int64_t)head * a.hq, a.ldq, a.dk, there);
+  dO.load_rows((const T*)a.dout + (clip * a.lq + row0) * a.lddo + (int64_t)head * a.hq, a.lddo, a.dk, there);
+  const int64_t crow = ((clip * a.lq + i) * a.heads + head) * a.dk;   // of the contiguous rows
+  const bool table_grad = BIAS && a.dtable;
+  if constexpr (BIAS) {
+    bias_line(mem, a, head);
+    if (table_grad) {
+      for (int d = tid; d < 4 * lines; d += 256) hist[d] = 0.f;
+      diag_start(hist + 4 * lines + wave * DIAG);
+    }
+  }
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < Frag<T, DK>::N; ++s) {
+    const uint32_t u[4] = {dO.x[s].x, dO.x[s].y, dO.x[s].z, dO.x[s].w};
+#pragma unroll
+    for (int f = 0; f < EPU; f += 4) {
+      const int c = (2 * s + h) * EPU + f;
+      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (there) {
+        if (a.dk % 4 == 0) {
+          if (c < a.dk) o = *(const f32x4*)(a.o32 + crow + c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < a.dk) o[e] = a.o32[crow + c + e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = sizeof(T) == 4 ? u[e] : e & 1 ? u[(f + e) >> 1] & 0xFFFF0000u : u[(f + e) >> 1] << 16;
+        delta = fmaf(__uint_as_float(x), o[e], delta);
+      }
+    }
+  }
+  delta = both_sum(delta);
+  if (split == 0 && h == 0 && i < a.lq) a.delta[srow] = delta;
+  f32x16 acc[DK / 32];
+#pragma unroll
+  for (int mb = 0; mb < DK / 32; ++mb) acc[mb] = zero16();
+  float past = 0.f, behind = 0.f;   // sums of ds at distances >= D, <= -D
+  float rest = 0.f, w_past = 0.f;   // (before 1 / l) sums of ds, and of weights at distances >= D
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     const uint4 *kimg = lds + buf * 2 * IMG, *vimg = kimg + IMG, *to = lds + (buf ^ 1) * 2 * IMG;
@@ -489,9 +484,6 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = row_bit(w4, r) ? s[r] : 0.f;
       }
-      if (rl == 0.f)   // a row that attends nothing
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = s[r] * (dp[r] - delta);
       if constexpr (BIAS) {
@@ -527,7 +519,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
     }
   }
   if (i < a.lq) {
-    if (rl == 0.f)
+    if (!there)
 #pragma unroll
       for (int mb = 0; mb < DK / 32; ++mb) acc[mb] = zero16();
     if (a.splits == 1) store_row<T, DK>((T*)a.dq + crow, acc, a.scale * rl, a.dk, a.vec_o);
@@ -539,13 +531,13 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
         rest = both_sum(rest) * rl;
         w_past = both_sum(w_past) * rl;
         if (h == 0 && i < a.lq) {
-          const int64_t all = (int64_t)a.n * a.heads * a.lq, at = ch * a.lq + i;
-          a.rest[2 * split * all + at] = rest;
-          a.rest[(2 * split + 1) * all + at] = w_past;
+          const int64_t all = (int64_t)a.n * a.heads * a.lq;
+          a.rest[2 * split * all + srow] = rest;
+          a.rest[(2 * split + 1) * all + srow] = w_past;
         }
       }
       __syncthreads();   // (a part without a tile has passed no barrier since the copies were cleared)
-      write_buckets(a, hist, past, behind, (int)(w % qt) * BT_ROWS, w);
+      write_buckets(a, hist, past, behind, first_row, w);
     }
   }
 }
@@ -560,30 +552,12 @@ __global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
   constexpr int KT = tile_rows<T, DK>(), IMG = KT * Img<T, DK>::UPR;
   extern __shared__ uint4 lds[];
   const int lines = 2 * a.distance + 1, D = a.distance;
-  float *line = (float*)(lds + 2 * IMG), *hist = line + (lines + 3) / 4 * 4;
-  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = tid >> 6;
-  const int qt = (a.lq + BT_ROWS - 1) / BT_ROWS;
-  const int64_t items = (int64_t)a.n * a.heads * qt, w = work_item(items);
+  float *mem = (float*)(lds + 2 * IMG), *line = mem + D + LINE_PAD, *hist = mem + line_floats(D);
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * qt, w = work_item(items);
   if (w >= items) return;
-  const int first = (int)(w % qt) * BT_ROWS, row0 = first + wave * 32, i = row0 + (lane & 31);
-  const int64_t ch = w / qt, clip = ch / a.heads, all = (int64_t)a.n * a.heads * a.lq;
-  const int head = (int)(ch % a.heads);
-  bias_line(line, a, head);
-  for (int d = tid; d < 4 * lines; d += 256) hist[d] = 0.f;
-  diag_start(hist + 4 * lines + wave * DIAG);
-  const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
-  Frag<T, DK> q;
-  q.load((const T*)a.q + clip * a.bq + (int64_t)i * a.ldq + (int64_t)head * a.hq, a.dk, there);
-  float m = INFINITY, rl = 0.f, e = 0.f, past = 0.f, near = 0.f;
-  if (there) {
-    const float2 st = *(const float2*)(a.stat + 2 * (ch * a.lq + i));
-    m = st.x;
-    rl = st.y;
-    for (int s = 0; s < a.splits; ++s) {
-      e += a.rest[2 * s * all + ch * a.lq + i];
-      past += a.rest[(2 * s + 1) * all + ch * a.lq + i];
-    }
-  }
+  const int first = (int)(w % qt) * BT_ROWS, row0 = first + wave * 32, i = row0 + (lane & 31), ch = w / qt, head = ch % a.heads;
+  const int64_t clip = ch / a.heads, all = (int64_t)a.n * a.heads * a.lq, srow = (int64_t)ch * a.lq + i;
   // keys within the distance of one of the block's queries: j - i - off in -D + 1 .. D - 1
   const int64_t j0 = (int64_t)first + a.off - D + 1, j1 = (int64_t)min(first + BT_ROWS, a.lq) - 1 + a.off + D;
   const int t0 = (int)max((int64_t)0, min(j0, (int64_t)a.lk)) / KT, t1 = (int)((max((int64_t)0, min(j1, (int64_t)a.lk)) + KT - 1) / KT);
@@ -594,6 +568,20 @@ __global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
   uint64_t next = __ballot(t0 < t1 ? mask_byte(mask, t0 * KT, KT, a.lk) : 0);
   if (t0 < t1) ks.load(kb, a.ldk, next, lds);
   int nb = t0 + 1 < t1 ? mask_byte(mask, (t0 + 1) * KT, KT, a.lk) : 0;
+  const bool mine = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
+  const float2 st = mine ? *(const float2*)(a.stat + 2 * srow) : make_float2(INFINITY, 0.f);
+  const float m = st.x, rl = st.y;
+  Frag<T, DK> q;
+  q.load_rows((const T*)a.q + clip * a.bq + (int64_t)row0 * a.ldq + (int64_t)head * a.hq, a.ldq, a.dk, mine);
+  float e = 0.f, past = 0.f, near = 0.f;
+  if (mine)
+    for (int s = 0; s < a.splits; ++s) {
+      e += a.rest[2 * s * all + srow];
+      past += a.rest[(2 * s + 1) * all + srow];
+    }
+  bias_line(mem, a, head);
+  for (int d = tid; d < 4 * lines; d += 256) hist[d] = 0.f;
+  diag_start(hist + 4 * lines + wave * DIAG);
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     const uint4* kimg = lds + buf * IMG;
@@ -625,9 +613,9 @@ __global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
     }
   }
   near = both_sum(near);
-  const bool mine = h == 0 && rl != 0.f;
-  const float behind = mine ? -e * (1.f - past - near) : 0.f;
-  past = mine ? -e * past : 0.f;
+  const bool counts = h == 0 && rl != 0.f;
+  const float behind = counts ? -e * (1.f - past - near) : 0.f;
+  past = counts ? -e * past : 0.f;
   __syncthreads();
   write_buckets(a, hist, past, behind, first, items * a.splits + w);
 }
@@ -655,21 +643,20 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1)
   constexpr int QT = tile_rows<T, DK>(), IMG = QT * Img<T, DK>::UPR;
   extern __shared__ uint4 lds[];
   // [2][q, do images], [2][3][QT] statistics (maximum, 1 / sum, delta), the bias line
-  float *stats = (float*)(lds + 4 * IMG), *line = stats + 6 * QT;
-  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = tid >> 6;
-  const int tiles = (a.lk + BT_ROWS - 1) / BT_ROWS;
-  const int64_t items = (int64_t)a.n * a.kv_heads * a.splits * tiles, w = work_item(items);
+  float *stats = (float*)(lds + 4 * IMG), *mem = stats + 6 * QT, *line = mem + a.distance + LINE_PAD;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t tiles = (a.lk + BT_ROWS - 1) / BT_ROWS, items = a.n * a.kv_heads * a.splits * tiles, w = work_item(items);
   if (w >= items) return;
-  const int key0 = (int)(w % tiles) * BT_ROWS, row0 = key0 + wave * 32, j = row0 + (lane & 31), split = (int)(w / tiles % a.splits);
-  const int64_t pair = w / tiles / a.splits, clip = pair / a.kv_heads;
-  const int kvh = (int)(pair % a.kv_heads), D = a.distance;
+  const int key0 = (int)(w % tiles) * BT_ROWS, row0 = key0 + wave * 32, j = row0 + (lane & 31), split = w / tiles % a.splits;
+  const int pair = w / tiles / a.splits, kvh = pair % a.kv_heads, D = a.distance;
+  const int64_t clip = pair / a.kv_heads;
   const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
   const bool any = __ballot(mask_byte(mask, key0, 64, a.lk)) | __ballot(mask_byte(mask, key0 + 64, 64, a.lk));
   const bool there = j < a.lk && (!mask || mask[j]);
   const bool live = __ballot(there);
   Frag<T, DK> k, v;
-  k.load((const T*)a.k + clip * a.bk + (int64_t)j * a.ldk + (int64_t)kvh * a.hk, a.dk, there);
-  v.load((const T*)a.v + clip * a.bv + (int64_t)j * a.ldv + (int64_t)kvh * a.hk, a.dk, there);
+  k.load_rows((const T*)a.k + clip * a.bk + (int64_t)row0 * a.ldk + (int64_t)kvh * a.hk, a.ldk, a.dk, there);
+  v.load_rows((const T*)a.v + clip * a.bv + (int64_t)row0 * a.ldv + (int64_t)kvh * a.hk, a.ldv, a.dk, there);
   f32x16 dk[DK / 32], dv[DK / 32];
 #pragma unroll
   for (int mb = 0; mb < DK / 32; ++mb) dk[mb] = dv[mb] = zero16();
@@ -714,7 +701,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1)
       if (t / qt != lined) {   // another head: its line, once all have done with the last one's
         __syncthreads();
         lined = t / qt;
-        bias_line(line, a, kvh * a.group + lined);
+        bias_line(mem, a, kvh * a.group + lined);
       }
     }
     tile_ready();
@@ -808,9 +795,9 @@ template <typename T, int DK, bool BIAS>
 struct Kernels {
   static constexpr int KT = tile_rows<T, DK>();
   static constexpr size_t IMAGES = 4 * (size_t)KT * Img<T, DK>::UPR * 16;
-  static size_t lines(const BtArgs& a) { return BIAS ? (2 * (size_t)a.distance + 1) * sizeof(float) : 0; }
+  static size_t lines(const BtArgs& a) { return BIAS ? line_floats(a.distance) * sizeof(float) : 0; }
 
-  static size_t table_lds(const BtArgs& a) { return 5 * lines(a) + 16 + 4 * DIAG * sizeof(float); }
+  static size_t table_lds(const BtArgs& a) { return lines(a) + (4 * (2 * (size_t)a.distance + 1) + 4 * DIAG) * sizeof(float); }
 
   static hipError_t fwd(const BtArgs& a, hipStream_t s) {
     static std::atomic<bool> done[64];
