@@ -389,10 +389,21 @@ __device__ __forceinline__ void diag_add(float* img, float* hist, const f32x16& 
   }
 }
 
-// XCD-aware block order: workgroups go to the 8 XCDs in turn; consecutive work items (the tiles that share
-// keys and values) go to one XCD, so that its L2 holds them once
-__device__ __forceinline__ uint32_t work_item(uint32_t items) { return (blockIdx.x & 7) * ((items + 7) / 8) + (blockIdx.x >> 3); }
-inline unsigned work_grid(int64_t items) { return (unsigned)((items + 7) / 8 * 8); }
+// XCD-aware block order: workgroups go to the 8 XCDs in turn.  The `each` items of a clip and kv head (the tiles that share keys
+// and values) go to one XCD, so that its L2 holds them once; the clips' kv heads are dealt to the XCDs in turn, so that
+// clips of other lengths mix on each.  Where they are few and do not divide, consecutive items go to an XCD.
+__host__ __device__ inline bool dealt(uint32_t items, uint32_t each) {
+  const uint32_t owners = items / each;
+  return owners % 8 == 0 || owners >= 64;
+}
+__device__ __forceinline__ uint32_t work_item(uint32_t items, uint32_t each) {
+  const uint32_t xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+  if (dealt(items, each)) return (xcd + 8 * (at / each)) * each + at % each;
+  return xcd * ((items + 7) / 8) + at;
+}
+inline unsigned work_grid(uint32_t items, uint32_t each) {
+  return dealt(items, each) ? (items / each + 7) / 8 * 8 * each : (items + 7) / 8 * 8;
+}
 
 struct Launch {
   hipError_t (*pack)(const BtArgs&, const void* src, int64_t ld, int64_t b, int rows, int heads, void* dst, hipStream_t);

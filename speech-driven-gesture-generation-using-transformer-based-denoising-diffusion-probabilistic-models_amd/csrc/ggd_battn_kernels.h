@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
   extern __shared__ uint4 lds[];
   float *mem = (float*)(lds + 4 * IMG), *line = mem + a.distance + LINE_PAD;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * qt, w = work_item(items);
+  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * qt, w = work_item(items, a.group * qt);
   if (w >= items) return;
   const int row0 = (int)(w % qt) * BT_ROWS + wave * 32, i = row0 + (lane & 31);
   const int ch = w / qt, head = ch % a.heads;   // clip heads + head
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1)
   extern __shared__ uint4 lds[];
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = a.group * a.lq, tiles = (rows + 31) / 32, kt = (a.lk + 31) / 32;
-  const uint32_t items = a.n * a.kv_heads * a.splits * tiles, w = work_item(items);
+  const uint32_t items = a.n * a.kv_heads * a.splits * tiles, w = work_item(items, a.splits * tiles);
   if (w >= items) return;
   const int tile = w % tiles, rest = w / tiles, split = rest % a.splits, pair = rest / a.splits, kvh = pair % a.kv_heads;
   const int64_t clip = pair / a.kv_heads;
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
   const int lines = 2 * a.distance + 1;
   float *mem = (float*)(lds + 4 * IMG), *line = mem + a.distance + LINE_PAD, *hist = mem + line_floats(a.distance);   // with a table gradient: [4][lines], and the diagonals' images
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * a.splits * qt, w = work_item(items);
+  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * a.splits * qt, w = work_item(items, a.group * a.splits * qt);
   if (w >= items) return;
   const int first_row = (int)(w % qt) * BT_ROWS, row0 = first_row + wave * 32, i = row0 + (lane & 31), split = w / qt % a.splits;
   const int ch = w / qt / a.splits, head = ch % a.heads, D = a.distance;
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
   const int lines = 2 * a.distance + 1, D = a.distance;
   float *mem = (float*)(lds + 2 * IMG), *line = mem + D + LINE_PAD, *hist = mem + line_floats(D);
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * qt, w = work_item(items);
+  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * qt, w = work_item(items, a.group * qt);
   if (w >= items) return;
   const int first = (int)(w % qt) * BT_ROWS, row0 = first + wave * 32, i = row0 + (lane & 31), ch = w / qt, head = ch % a.heads;
   const int64_t clip = ch / a.heads, all = (int64_t)a.n * a.heads * a.lq, srow = (int64_t)ch * a.lq + i;
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1)
   // [2][q, do images], [2][3][QT] statistics (maximum, 1 / sum, delta), the bias line
   float *stats = (float*)(lds + 4 * IMG), *mem = stats + 6 * QT, *line = mem + a.distance + LINE_PAD;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t tiles = (a.lk + BT_ROWS - 1) / BT_ROWS, items = a.n * a.kv_heads * a.splits * tiles, w = work_item(items);
+  const uint32_t tiles = (a.lk + BT_ROWS - 1) / BT_ROWS, items = a.n * a.kv_heads * a.splits * tiles, w = work_item(items, a.splits * tiles);
   if (w >= items) return;
   const int key0 = (int)(w % tiles) * BT_ROWS, row0 = key0 + wave * 32, j = row0 + (lane & 31), split = w / tiles % a.splits;
   const int pair = w / tiles / a.splits, kvh = pair % a.kv_heads, D = a.distance;
@@ -803,8 +803,8 @@ struct Kernels {
     static std::atomic<bool> done[64];
     const size_t lds = IMAGES + lines(a);
     if (const hipError_t e = allow_lds(bt_fwd_kernel<T, DK, BIAS>, lds, done)) return e;
-    const int64_t items = (int64_t)a.n * a.heads * ((a.lq + BT_ROWS - 1) / BT_ROWS);
-    hipLaunchKernelGGL((bt_fwd_kernel<T, DK, BIAS>), dim3(work_grid(items)), dim3(256), lds, s, a);
+    const uint32_t each = a.group * ((a.lq + BT_ROWS - 1) / BT_ROWS);
+    hipLaunchKernelGGL((bt_fwd_kernel<T, DK, BIAS>), dim3(work_grid(a.n * a.kv_heads * each, each)), dim3(256), lds, s, a);
     return hipGetLastError();
   }
   static hipError_t few(const BtArgs& a, hipStream_t s) {
@@ -812,18 +812,18 @@ struct Kernels {
     // the four waves' images, which then hold the four parts of o (f32) and 384 statistics
     const size_t lds = std::max<size_t>(4 * 2 * 32 * Img<T, DK>::UPR * 16, 4 * 32 * DK * sizeof(float)) + 1536;
     if (const hipError_t e = allow_lds(bt_few_kernel<T, DK, BIAS>, lds, done)) return e;
-    const int64_t rows = ((int64_t)a.group * a.lq + 31) / 32 * a.n * a.kv_heads;
-    hipLaunchKernelGGL((bt_few_kernel<T, DK, BIAS>), dim3(work_grid(rows * a.splits)), dim3(256), lds, s, a);
+    const uint32_t tiles = (a.group * a.lq + 31) / 32, rows = tiles * a.n * a.kv_heads;
+    hipLaunchKernelGGL((bt_few_kernel<T, DK, BIAS>), dim3(work_grid(rows * a.splits, a.splits * tiles)), dim3(256), lds, s, a);
     if (a.splits > 1)
-      hipLaunchKernelGGL((bt_join_kernel<T, DK>), dim3((unsigned)((rows * 32 + 1024 / DK - 1) / (1024 / DK))), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((bt_join_kernel<T, DK>), dim3((rows * 32 + 1024 / DK - 1) / (1024 / DK)), dim3(256), 0, s, a);
     return hipGetLastError();
   }
   static hipError_t dq(const BtArgs& a, hipStream_t s) {
     static std::atomic<bool> done[64];
     const size_t lds = IMAGES + (a.dtable ? table_lds(a) : lines(a));
     if (const hipError_t e = allow_lds(bt_dq_kernel<T, DK, BIAS>, lds, done)) return e;
-    const int qt = (a.lq + BT_ROWS - 1) / BT_ROWS;
-    hipLaunchKernelGGL((bt_dq_kernel<T, DK, BIAS>), dim3(work_grid((int64_t)a.n * a.heads * qt * a.splits)), dim3(256), lds, s, a);
+    const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, each = a.group * qt;
+    hipLaunchKernelGGL((bt_dq_kernel<T, DK, BIAS>), dim3(work_grid(a.n * a.kv_heads * each * a.splits, each * a.splits)), dim3(256), lds, s, a);
     if (const hipError_t e = hipGetLastError()) return e;
     if constexpr (BIAS) {
       if (a.dtable) {
@@ -831,9 +831,9 @@ struct Kernels {
           static std::atomic<bool> rest_done[64];
           const size_t rest_lds = IMAGES / 2 + table_lds(a);
           if (const hipError_t e = allow_lds(bt_table_rest_kernel<T, DK>, rest_lds, rest_done)) return e;
-          hipLaunchKernelGGL((bt_table_rest_kernel<T, DK>), dim3(work_grid((int64_t)a.n * a.heads * qt)), dim3(256), rest_lds, s, a);
+          hipLaunchKernelGGL((bt_table_rest_kernel<T, DK>), dim3(work_grid(a.n * a.kv_heads * each, each)), dim3(256), rest_lds, s, a);
         }
-        hipLaunchKernelGGL(bt_table_kernel, dim3(a.heads * a.n_buckets), dim3(64), 0, s, a, qt * a.splits, sizeof(T) == 2 ? qt : 0);
+        hipLaunchKernelGGL(bt_table_kernel, dim3(a.heads * a.n_buckets), dim3(64), 0, s, a, (int)(qt * a.splits), sizeof(T) == 2 ? (int)qt : 0);
         if (const hipError_t e = hipGetLastError()) return e;
       }
     }
@@ -843,8 +843,8 @@ struct Kernels {
     static std::atomic<bool> done[64];
     const size_t lds = IMAGES + 6 * KT * sizeof(float) + lines(a);
     if (const hipError_t e = allow_lds(bt_dkv_kernel<T, DK, BIAS>, lds, done)) return e;
-    const int64_t items = (int64_t)a.n * a.kv_heads * ((a.lk + BT_ROWS - 1) / BT_ROWS) * a.splits;
-    hipLaunchKernelGGL((bt_dkv_kernel<T, DK, BIAS>), dim3(work_grid(items)), dim3(256), lds, s, a);
+    const uint32_t each = (a.lk + BT_ROWS - 1) / BT_ROWS * a.splits;
+    hipLaunchKernelGGL((bt_dkv_kernel<T, DK, BIAS>), dim3(work_grid(a.n * a.kv_heads * each, each)), dim3(256), lds, s, a);
     if (const hipError_t e = hipGetLastError()) return e;
     if (a.splits == 1) return hipSuccess;
     const int64_t all = (int64_t)a.n * a.lk * a.kv_heads * a.dk;
