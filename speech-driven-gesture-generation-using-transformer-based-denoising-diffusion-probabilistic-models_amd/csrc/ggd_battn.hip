@@ -81,6 +81,10 @@ int few_splits(const BtArgs& a) {
   return parts(blocks, (a.lk + 31) / 32, 8, slots(a, 64, 32));
 }
 int tile(const BtArgs& a) { return a.dtype == GGD_TR_F32 && a.dk > 64 ? 32 : 64; }
+int fwd_splits(const BtArgs& a) {
+  if (few_rows(a)) return few_splits(a);
+  return parts((int64_t)a.n * a.heads * ((a.lq + BT_ROWS - 1) / BT_ROWS), (a.lk + tile(a) - 1) / tile(a), 4, slots(a, 128, 64));
+}
 int dq_splits(const BtArgs& a) {
   return parts((int64_t)a.n * a.heads * ((a.lq + BT_ROWS - 1) / BT_ROWS), (a.lk + tile(a) - 1) / tile(a), 4, slots(a, 128, 64));
 }
@@ -114,8 +118,8 @@ Space forward_space(const BtArgs& a) {
   Space s{};
   const Packed p = packed_space(a);
   if (packed(a, false)) s.pack = p.q + 2 * p.k;
-  if (few_rows(a) && few_splits(a) > 1)
-    s.part = up(((int64_t)a.group * a.lq + 31) / 32 * 32 * a.n * a.kv_heads * few_splits(a) * (dk_class(a) + 4) * 4);
+  if (const int splits = fwd_splits(a); splits > 1)
+    s.part = up(((int64_t)a.group * a.lq + 31) / 32 * 32 * a.n * a.kv_heads * splits * (dk_class(a) + 4) * 4);
   return s;
 }
 
@@ -170,7 +174,7 @@ int ggd_tr_battn_fwd(const ggd_tr_battn_args* args, void* stream) {
   if (!aligned(a.stat, 8)) return -1;
   a.vec_o = a.dk % 4 == 0 && a.ldo % 4 == 0 && a.bo % 4 == 0 && aligned(a.o, 4 * esize(a)) && aligned(a.o32, 16);
   const bool few = few_rows(a);
-  a.splits = few ? few_splits(a) : 1;
+  a.splits = fwd_splits(a);
   a.part = (float*)((char*)a.ws + space.pack);
   const hipStream_t s = (hipStream_t)stream;
   if (rows(a, false, s) != hipSuccess) return -3;

@@ -105,46 +105,58 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
   extern __shared__ uint4 lds[];
   float *mem = (float*)(lds + 4 * IMG), *line = mem + a.distance + LINE_PAD;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * qt, w = work_item(items, a.group * qt);
+  const uint32_t qt = (a.lq + BT_ROWS - 1) / BT_ROWS, items = a.n * a.heads * a.splits * qt, w = work_item(items, a.group * a.splits * qt);
   if (w >= items) return;
-  const int row0 = (int)(w % qt) * BT_ROWS + wave * 32, i = row0 + (lane & 31);
-  const int ch = w / qt, head = ch % a.heads;   // clip heads + head
+  const int row0 = (int)(w % qt) * BT_ROWS + wave * 32, i = row0 + (lane & 31), split = w / qt % a.splits;
+  const int ch = w / qt / a.splits, head = ch % a.heads;   // clip heads + head
   const int64_t clip = ch / a.heads;
-  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.hk;
-  const T* vb = (const T*)a.v + clip * a.bv + (int64_t)(head / a.group) * a.hk;
+  const int kt = (a.lk + KT - 1) / KT, per = (kt + a.splits - 1) / a.splits, t0 = split * per, t1 = min(kt, t0 + per);
+  const T* kb = (const T*)a.k + clip * a.bk + (int64_t)(head / a.group) * a.hk + (int64_t)t0 * KT * a.ldk;
+  const T* vb = (const T*)a.v + clip * a.bv + (int64_t)(head / a.group) * a.hk + (int64_t)t0 * KT * a.ldv;
   const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
   Tile<T, DK, KT> ks, vs;
   ks.start(a.ldk, a.dk);
   vs.start(a.ldv, a.dk);
-  uint64_t bits = __ballot(mask_byte(mask, 0, KT, a.lk));
-  ks.load(kb, a.ldk, bits, lds);
-  vs.load(vb, a.ldv, bits, lds + IMG);
-  int nb = mask_byte(mask, KT, KT, a.lk);
+  uint64_t next = __ballot(t0 < t1 ? mask_byte(mask, t0 * KT, KT, a.lk) : 0);
+  if (t0 < t1) {
+    ks.load(kb, a.ldk, next, lds);
+    vs.load(vb, a.ldv, next, lds + IMG);
+  }
+  int nb = t0 + 1 < t1 ? mask_byte(mask, (t0 + 1) * KT, KT, a.lk) : 0;
   const bool there = i < a.lq && (!a.q_mask || a.q_mask[clip * a.bq_mask + i]);
   Frag<T, DK> q;
   q.load_rows((const T*)a.q + clip * a.bq + (int64_t)row0 * a.ldq + (int64_t)head * a.hq, a.ldq, a.dk, there);
   if constexpr (BIAS) bias_line(mem, a, head);
   Softmax<DK> sm;
   sm.start();
-  const int nt = (a.lk + KT - 1) / KT;
-  for (int t = 0; t < nt; ++t) {
-    const uint4 *kimg = lds + (t & 1) * 2 * IMG, *vimg = kimg + IMG, *to = lds + (~t & 1) * 2 * IMG;
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    const uint4 *kimg = lds + buf * 2 * IMG, *vimg = kimg + IMG, *to = lds + (buf ^ 1) * 2 * IMG;
     tile_ready();
-    const uint64_t next = __ballot(nb);
+    const uint64_t bits = next;
+    next = __ballot(nb);
     kb += KT * a.ldk;
     vb += KT * a.ldv;
-    if (t + 1 < nt) {   // (no load may be under way when the block ends)
+    if (t + 1 < t1) {   // (no load may be under way when the block ends)
       ks.load(kb, a.ldk, next, to);
       vs.load(vb, a.ldv, next, to + IMG);
     }
-    nb = mask_byte(mask, (t + 2) * KT, KT, a.lk);
+    nb = t + 2 < t1 ? mask_byte(mask, (t + 2) * KT, KT, a.lk) : 0;
     if (bits && row0 < a.lq) {
       const int first = t * KT - a.off;
       attend<T, DK, BIAS, KT / 32>(sm, kimg, vimg, q, bits, a, line, first + 4 * h - i, first - (row0 + 31), first + 31 - row0);
     }
-    bits = next;
   }
   sm.template finish<T>();
+  if (a.splits > 1) {   // a part of the keys, laid out for bt_join_kernel
+    if (i >= a.lq) return;
+    const int tiles = (a.group * a.lq + 31) / 32;
+    const int64_t all = (int64_t)a.n * a.kv_heads * tiles * 32;
+    const int64_t p = split * all + (clip * a.kv_heads + head / a.group) * tiles * 32 + (int64_t)(head % a.group) * a.lq + i;
+    store_row<float, DK>(a.part + p * DK, sm.o, 1.f, DK, true);
+    if (h == 0) *(f32x4*)(a.part + a.splits * all * DK + 4 * p) = f32x4{sm.m, sm.l, sm.lr, 0.f};
+    return;
+  }
   const bool some = there && sm.lr != 0.f;
   const float inv = some ? 1.0f / sm.lr : 0.f;
   if (i >= a.lq) return;
@@ -799,12 +811,17 @@ struct Kernels {
 
   static size_t table_lds(const BtArgs& a) { return lines(a) + (4 * (2 * (size_t)a.distance + 1) + 4 * DIAG) * sizeof(float); }
 
+  static void join(const BtArgs& a, hipStream_t s) {
+    const uint32_t rows = (a.group * a.lq + 31) / 32 * 32 * a.n * a.kv_heads;
+    hipLaunchKernelGGL((bt_join_kernel<T, DK>), dim3((rows + 1024 / DK - 1) / (1024 / DK)), dim3(256), 0, s, a);
+  }
   static hipError_t fwd(const BtArgs& a, hipStream_t s) {
     static std::atomic<bool> done[64];
     const size_t lds = IMAGES + lines(a);
     if (const hipError_t e = allow_lds(bt_fwd_kernel<T, DK, BIAS>, lds, done)) return e;
-    const uint32_t each = a.group * ((a.lq + BT_ROWS - 1) / BT_ROWS);
+    const uint32_t each = a.group * ((a.lq + BT_ROWS - 1) / BT_ROWS) * a.splits;
     hipLaunchKernelGGL((bt_fwd_kernel<T, DK, BIAS>), dim3(work_grid(a.n * a.kv_heads * each, each)), dim3(256), lds, s, a);
+    if (a.splits > 1) join(a, s);
     return hipGetLastError();
   }
   static hipError_t few(const BtArgs& a, hipStream_t s) {
@@ -814,8 +831,7 @@ struct Kernels {
     if (const hipError_t e = allow_lds(bt_few_kernel<T, DK, BIAS>, lds, done)) return e;
     const uint32_t tiles = (a.group * a.lq + 31) / 32, rows = tiles * a.n * a.kv_heads;
     hipLaunchKernelGGL((bt_few_kernel<T, DK, BIAS>), dim3(work_grid(rows * a.splits, a.splits * tiles)), dim3(256), lds, s, a);
-    if (a.splits > 1)
-      hipLaunchKernelGGL((bt_join_kernel<T, DK>), dim3((rows * 32 + 1024 / DK - 1) / (1024 / DK)), dim3(256), 0, s, a);
+    if (a.splits > 1) join(a, s);
     return hipGetLastError();
   }
   static hipError_t dq(const BtArgs& a, hipStream_t s) {
