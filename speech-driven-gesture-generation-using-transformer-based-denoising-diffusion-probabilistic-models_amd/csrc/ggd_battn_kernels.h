@@ -376,13 +376,34 @@ __device__ __forceinline__ void write_buckets(const BtArgs& a, float* hist, floa
     which[d] = bucket_of(a, d);
   }
   __syncthreads();
-  for (int b = wave; b < a.n_buckets; b += 4) {
-    float x = 0.f;
-    for (int d = d0 + lane; d <= d1; d += 64) x += which[d] == b ? hist[d] : 0.f;
+  auto leave = [&](int b, float x) {
     x = group_sum<16>(x);
     x += __shfl_xor(x, 16);
     x = both_sum(x);
     if (lane == 0) a.dtab[row * a.n_buckets + b] = x;
+  };
+  constexpr int HELD = 8;   // distances a lane holds: most blocks have no more
+  if (d1 - d0 < 64 * HELD) {
+    float v[HELD];
+    int of[HELD];
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      const int d = d0 + 64 * k + lane;
+      v[k] = d <= d1 ? hist[d] : 0.f;
+      of[k] = d <= d1 ? which[d] : -1;
+    }
+    for (int b = wave; b < a.n_buckets; b += 4) {
+      float x = 0.f;
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) x += of[k] == b ? v[k] : 0.f;
+      leave(b, x);
+    }
+  } else {
+    for (int b = wave; b < a.n_buckets; b += 4) {
+      float x = 0.f;
+      for (int d = d0 + lane; d <= d1; d += 64) x += which[d] == b ? hist[d] : 0.f;
+      leave(b, x);
+    }
   }
 }
 
@@ -585,12 +606,13 @@ __global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
   const float m = st.x, rl = st.y;
   Frag<T, DK> q;
   q.load_rows((const T*)a.q + clip * a.bq + (int64_t)row0 * a.ldq + (int64_t)head * a.hq, a.ldq, a.dk, mine);
-  float e = 0.f, past = 0.f, near = 0.f;
+  float e = 0.f, past = 0.f, near = 0.f;   // near: weights before 1 / l
   if (mine)
     for (int s = 0; s < a.splits; ++s) {
       e += a.rest[2 * s * all + srow];
       past += a.rest[(2 * s + 1) * all + srow];
     }
+  const float back = -e * rl;   // (a row that attends nothing: 0, and its maximum is infinite)
   bias_line(mem, a, head);
   for (int d = tid; d < 4 * lines; d += 256) hist[d] = 0.f;
   diag_start(hist + 4 * lines + wave * DIAG);
@@ -612,19 +634,30 @@ __global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
       f32x16 s = zero16();
       mma_rows<T, DK>(s, kimg, 32 * b, q);
       add_bias<1>(s, line, a.c, rel, D, lo, hi);
-      const uint32_t w4 = w32 >> (4 * h);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] - m);
+      if (w32 != 0xFFFFFFFFu) {
+        const uint32_t w4 = w32 >> (4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = row_bit(w4, r) ? s[r] : 0.f;
+      }
+      if (lo <= -D || hi >= D) {   // places past the distance are not this kernel's
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = rel + 8 * (r >> 2) + (r & 3);
+          s[r] = d < D && d > -D ? s[r] : 0.f;
+        }
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int d = rel + 8 * (r >> 2) + (r & 3);
-        const float p = rl != 0.f && row_bit(w4, r) && d < D && d > -D ? __builtin_amdgcn_exp2f(s[r] - m) * rl : 0.f;
-        near += p;
-        s[r] = -e * p;
+        near += s[r];
+        s[r] *= back;
       }
       float none = 0.f;
       diag_add(hist + 4 * lines + wave * DIAG, hist + wave * lines + D, s, at - row0, D, none, none);
     }
   }
-  near = both_sum(near);
+  near = both_sum(near) * rl;
   const bool counts = h == 0 && rl != 0.f;
   const float behind = counts ? -e * (1.f - past - near) : 0.f;
   past = counts ? -e * past : 0.f;
