@@ -12,6 +12,7 @@ streams and captured graphs share nothing; a pass that was run once may be captu
 A wrong shape, type or device raises ValueError before anything is launched.  The checks, the allocations and
 the autograd nodes are in csrc/ggd_blocks.cpp.
 """
+import numpy as np
 import torch as th
 
 from . import native
@@ -46,18 +47,19 @@ class RelativeBuckets:
         if not side // 2 < max_distance <= MAX_DISTANCE:
             raise ValueError(f"RelativeBuckets: max_distance {max_distance}: more than {side // 2}, up to {MAX_DISTANCE}")
         self.n_buckets, self.max_distance, self.both_sides = n_buckets, max_distance, bool(both_sides)
-        near, steps, of = side // 2, side - side // 2, []
-        passed = 0
-        for d in range(max_distance + 1):
-            if d < near:
-                of.append(d)
-                continue
-            while passed + 1 < steps and d ** steps >= near ** (steps - passed - 1) * max_distance ** (passed + 1):
-                passed += 1
-            of.append(near + passed)
-        behind = [of[d] for d in range(max_distance, 0, -1)]
-        ahead = [side + of[d] if both_sides else 0 for d in range(1, max_distance + 1)]
-        self.buckets = th.tensor(behind + [of[0]] + ahead, dtype=th.int32)   # of d = -max_distance .. max_distance
+        near, steps = side // 2, side - side // 2
+        starts = list(range(near + 1))   # of each bucket of a side; then the least d with d^steps >= near^(steps - k) most^k
+        for k in range(1, steps):
+            border = near ** (steps - k) * max_distance ** k
+            d = round(near * (max_distance / near) ** (k / steps))
+            while d ** steps < border:
+                d += 1
+            while (d - 1) ** steps >= border:
+                d -= 1
+            starts.append(d)
+        of = np.repeat(np.arange(side, dtype=np.int32), np.diff([*starts, max_distance + 1]))   # of |d| = 0 .. max_distance
+        ahead = of[1:] + side if both_sides else np.zeros(max_distance, np.int32)
+        self.buckets = th.from_numpy(np.concatenate([of[:0:-1], of[:1], ahead]))   # of d = -max_distance .. max_distance
         self._on = {}
         if th.device(device).type != "cpu":
             self.on(th.device(device))
