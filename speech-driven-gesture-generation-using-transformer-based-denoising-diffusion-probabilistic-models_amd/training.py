@@ -37,6 +37,7 @@ import torch as th
 import torch.nn.functional as F
 
 from . import native
+from .blocks import cross_attention
 from .weights import parameter_shapes
 
 EW_RELU2, EW_RELU2_BWD, EW_SILU, EW_SILU_BWD, EW_ADD = 0, 1, 2, 3, 4   # include/ggd_train.h
@@ -228,6 +229,18 @@ class _Attention(th.autograd.Function):
         _ok(_lib().ggd_tr_attention_bwd(n, H, Lq, Lk, W // H, ctx.scale, _p(q), W, _p(k), _p(v), W, _p(do), W, _p(dq),
                                         _p(dk_), _p(dv), _s(q)), "attention bwd")
         return dq, dk_, dv, None, None
+
+
+def attention(q, k, v, heads, scale):
+    """softmax(Q K^T scale) V of (n, L, heads dk) rows: one block a clip and head where its rows and
+    probabilities fit the LDS (the kernels of csrc/ggd_train.hip), cross_attention's tiles for longer clips --
+    at dk = 64, from 112 frames over as many memory rows on where a backward pass follows."""
+    Lq, Lk, dk = q.shape[1], k.shape[1], q.shape[2] // heads
+    back = th.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    floats = ((2 * Lq + 2 * Lk) * dk + Lq if back else (Lq + 2 * Lk) * dk) + Lq * Lk   # att_lds_bytes there
+    if max(Lq, Lk) <= 256 and 4 * floats <= 160 * 1024:
+        return _Attention.apply(q, k, v, heads, scale)
+    return cross_attention(q, k, v, heads, scale=scale)
 
 
 def _ew(op, a, b=None):
@@ -653,7 +666,7 @@ class TrainableModel:
             return _SeqConv.apply(y.contiguous(), P[f"{pre}.{w}.1.conv.weight"], P[f"{pre}.{w}.1.conv.bias"], H)
 
         q, k, v = heads(q_in, "query"), heads(kv_in, "key"), heads(kv_in, "value")
-        o = _Attention.apply(q, k, v, H, 1.0 / math.sqrt(d // H))
+        o = attention(q, k, v, H, 1.0 / math.sqrt(d // H))
         return linear(o, P[f"{pre}.output.weight"], P[f"{pre}.output.bias"])
 
     # -- the HA2G encoder in train mode (ResNetSE34V2.py:118-188), NHWC ---------------------------
