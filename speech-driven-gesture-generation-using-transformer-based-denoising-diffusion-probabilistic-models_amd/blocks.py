@@ -7,7 +7,8 @@ matrices, (n, L, heads dk) rows of heads; each is hand-written HIP kernels behin
 and backward, in f32 or bf16 with sums, softmax and statistics in f32.  Under torch.no_grad() a call
 keeps nothing for a backward pass.  Gradients come once: a second derivative raises.  Everything is issued on the
 current stream of the inputs' device, with workspaces from torch's allocator, so that calls on several
-streams and captured graphs share nothing; a pass that was run once may be captured.
+streams and captured graphs share nothing; a pass that was run once may be captured.  A captured call with
+gradients wants leaves of which no eager graph is alive (a loss kept from before, say), and is refused else.
 
 A wrong shape, type or device raises ValueError before anything is launched.  The checks, the allocations and
 the autograd nodes are in csrc/ggd_blocks.cpp.

@@ -9,6 +9,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -68,6 +69,24 @@ OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : std::null
 Tensor workspace(int64_t bytes, const Tensor& like) { return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+// In a captured call: a leaf whose gradient accumulator another stream made -- an eager graph of it is alive -- would draw that stream
+// into the capture when its gradient arrives, past any error that could be caught.
+void check_capture(const char* what, std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad()) continue;
+    const at::TensorBase& leaf = t.is_view() ? t._base() : t;
+    if (!leaf.requires_grad() || !leaf.is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
+    if (!accumulator) continue;
+    const auto made = accumulator->stream();
+    const auto stream = c10::hip::getCurrentHIPStream(t.device().index());
+    if (!made || made->id() == stream.id()) continue;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream.stream(), &status) == hipSuccess && status == hipStreamCaptureStatusActive)
+      refuse(what, "captured while an eager graph of an input is alive; let go of that graph's outputs first");
+  }
+}
 
 // Gradients come once: where a graph of them is asked for, one that raises when it is used.
 variable_list once(variable_list grads, const char* what) {
@@ -194,11 +213,12 @@ Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tenso
     refuse(what, "q, k and v have to be of one type, float32 or bfloat16");
   if (q.size(1) > 1 << 28 || k.size(1) > 1 << 28 || n > INT32_MAX || heads > INT32_MAX) refuse(what, "unsupported shape");
   const double scale = sc.value_or(1.0 / std::sqrt((double)dk));
-  if (!(scale > 0.0 && scale <= 1e30)) refuse(what, "scale ", scale, " has to be positive");
+  if (!((float)scale > 0.f && scale <= 1e30)) refuse(what, "scale ", scale, " has to be positive");
   Inputs in{rows(q), rows(k), rows(v), Tensor(), mask_rows(what, "mask", mask, n, k.size(1)), mask_rows(what, "q_mask", q_mask, n, q.size(1)),
             or_none(buckets), heads, kv_heads, offset, scale};
   if (table) in.table = table->contiguous();
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (table && table->requires_grad()));
+  if (grad) check_capture(what, {q, k, v, or_none(table)});
   if (grad) return Attention::apply(in.q, in.k, in.v, given(in.table), given(in.mask), given(in.q_mask), given(in.buckets), heads, kv_heads, scale, offset);
   Tensor stat, o32;
   return attend(in, false, stat, o32);
@@ -300,6 +320,7 @@ std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre
   if (d < 1 || d > 8192) refuse(what, "rows of ", d, " elements: 1 to 8192");
   variable_list w{or_none(post_g), or_none(post_b), or_none(pre_g), or_none(pre_b)};
   bool grad = h.requires_grad() || y.requires_grad() || (gate_in && gate_in->requires_grad());
+  if (at::GradMode::is_enabled()) check_capture(what, {h, y, or_none(gate_in), w[0], w[1], w[2], w[3]});
   for (Tensor& t : w)
     if (t.defined()) {
       beside(what, "a weight or bias", t, h);
@@ -307,7 +328,7 @@ std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre
       grad = grad || t.requires_grad();
       t = t.contiguous();
     }
-  if (!std::isfinite(scale) || !std::isfinite(eps) || !(eps > 0.0)) refuse(what, "scale ", scale, " has to be finite, eps ", eps, " positive");
+  if (!std::isfinite((float)scale) || !std::isfinite((float)eps) || !((float)eps > 0.f)) refuse(what, "scale ", scale, " has to be finite, eps ", eps, " positive");
   Shape g{h.numel() / d, d, 1, kind, scale, eps};
   Tensor gate = or_none(gate_in);
   if (gate.defined()) g.gate_rows = gate_rows_of(what, gate, h);

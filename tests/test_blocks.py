@@ -85,7 +85,9 @@ BAD = [dict(n=-1), dict(heads=0), dict(kv_heads=0), dict(heads=3), dict(lq=0), d
        dict(table=1 << 20), dict(buckets=1 << 20), dict(table=1 << 20, buckets=1 << 20, n_buckets=0, distance=4),
        dict(table=1 << 20, buckets=1 << 20, n_buckets=4, distance=0)]
 UNSUPPORTED = [dict(dk=129), dict(lq=(1 << 28) + 1), dict(lk=(1 << 28) + 1), dict(table=1 << 20, buckets=1 << 20, n_buckets=1025, distance=4),
-               dict(table=1 << 20, buckets=1 << 20, n_buckets=8, distance=2048), dict(n=1 << 20, lq=1 << 20), dict(n=1, heads=64, kv_heads=1, lq=1 << 27)]
+               dict(table=1 << 20, buckets=1 << 20, n_buckets=8, distance=2048), dict(n=1 << 20, lq=1 << 20), dict(n=1, heads=64, kv_heads=1, lq=1 << 27),
+               dict(n=1 << 30, heads=1 << 30, kv_heads=1 << 30, lq=1 << 28),   # (a product past 64 bits)
+               dict(n=1, heads=1 << 17, kv_heads=1 << 17, table=1 << 20, buckets=1 << 20, n_buckets=1024, distance=2047)]
 
 
 def test_attention_entry_refusals(native):

@@ -383,6 +383,53 @@ def test_attention_captured_and_replayed(pkg):
         assert all(th.equal(a, b) for a, b in zip(o2, want))
 
 
+def test_a_capture_beside_an_eager_graph_is_refused(pkg):
+    """A gradient of the captured pass would draw the eager graph's stream into the capture: refused before, and
+    allowed once that graph is gone."""
+    x = attention_inputs("f32", 1, 9, 9, 2, 2, 16)[0][0].requires_grad_()
+    w = th.ones(32, device="cuda", requires_grad=True)
+    with th.no_grad():
+        pkg.cross_attention(x, x, x, 2), pkg.residual_norm(x, x, (w, None))
+
+    def attend(t):
+        return pkg.cross_attention(t, t, t, 2)
+
+    for call in (lambda: attend(x), lambda: attend(x[:, 1:]), lambda: pkg.residual_norm(x, x.detach(), (w, None))[1],
+                 lambda: pkg.residual_norm(x.detach(), x.detach(), (w, None))[1]):
+        alive = call()
+        with pytest.raises(ValueError, match="eager graph"):
+            with th.cuda.graph(th.cuda.CUDAGraph()):
+                x.detach() + 1   # (a capture of something)
+                call()
+        with th.no_grad():   # without gradients there is nothing to refuse
+            graph = th.cuda.CUDAGraph()
+            with th.cuda.graph(graph):
+                o = call()
+        graph.replay()
+        th.cuda.synchronize()
+        assert th.equal(o, alive.detach())
+        del alive
+        graph = th.cuda.CUDAGraph()
+        with th.cuda.graph(graph):
+            o = call()
+            grads = th.autograd.grad(o, [t for t in (x, w) if o.grad_fn is not None], th.ones_like(o), allow_unused=True)
+        graph.replay()
+        th.cuda.synchronize()
+        want = call()
+        assert th.equal(o.detach(), want.detach())
+        for a, b in zip(grads, th.autograd.grad(want, [x, w], th.ones_like(want), allow_unused=True)):
+            assert (a is None) == (b is None) and (a is None or th.equal(a, b))
+        del o, want, grads
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_widest_heads_with_the_longest_distance(pkg, dtype):
+    """The largest histograms and images that share the LDS, and the most buckets."""
+    buckets = pkg.RelativeBuckets(1024, 2047)
+    ins, do, _ = attention_inputs(dtype, 1, 150, 140, 2, 1, 128, n_buckets=1024)
+    check_attention(pkg, ins, do, 2, 1, buckets=buckets, offset=-3)
+
+
 def test_attention_leaves_other_memory_alone(pkg):
     """Outputs lie in fresh tensors: inputs stay as they are, and so does what lies around a view's rows."""
     ins, do, g = attention_inputs("bf16", 2, 33, 45, 2, 1, 24)
@@ -652,7 +699,7 @@ def test_refusals(pkg):
                  lambda: cross(q, k.cpu(), k, 4, kv_heads=2), lambda: cross(z(1, 2, 130), z(1, 2, 130), z(1, 2, 130), 1),
                  lambda: cross(q, k, k, 4, kv_heads=2, mask=keep.float()), lambda: cross(q, k, k, 4, kv_heads=2, mask=keep[:, :4]),
                  lambda: cross(q, k, k, 4, kv_heads=2, mask=keep.cpu()), lambda: cross(q, k, k, 4, kv_heads=2, q_mask=keep),
-                 lambda: cross(q, k, k, 4, kv_heads=2, scale=0.0), lambda: cross(q, k, k, 4, kv_heads=2, scale=math.nan),
+                 lambda: cross(q, k, k, 4, kv_heads=2, scale=0.0), lambda: cross(q, k, k, 4, kv_heads=2, scale=1e-60), lambda: cross(q, k, k, 4, kv_heads=2, scale=math.nan),
                  lambda: rel(q, k, k, 4, b, None, kv_heads=2), lambda: rel(q, k, k, 4, None, table, kv_heads=2),
                  lambda: rel(q, k, k, 4, b, table[:7], kv_heads=2), lambda: rel(q, k, k, 4, b, table.double(), kv_heads=2),
                  lambda: rel(q, k, k, 4, b, table.cpu(), kv_heads=2)):
@@ -665,6 +712,7 @@ def test_refusals(pkg):
                  lambda: norm(h, h.bfloat16(), (w, w)), lambda: norm(h.half(), h.half(), (w, w)), lambda: norm(h, h, (w[:8], w)),
                  lambda: norm(h, h, (w.bfloat16(), w)), lambda: norm(h, h, (w, w), gate=z(3, 1, 16)), lambda: norm(h, h, (w, w), gate=z(16).bfloat16()),
                  lambda: norm(h, h, (w, w), gate=z(1, 2, 3, 16)), lambda: norm(h, h, (w, w), kind="batch"), lambda: norm(h, h, (w, w), eps=0.0),
+                 lambda: norm(h, h, (w, w), eps=1e-60), lambda: norm(h, h, (w, w), scale=1e60),
                  lambda: norm(h, h, (w, w), scale=math.inf), lambda: norm(h, h, w), lambda: norm(h, h.cpu(), (w, w)),
                  lambda: norm(z(1, 8193), z(1, 8193), (z(8193), None)), lambda: norm(z(2, 0), z(2, 0), (z(0), None))):
         with pytest.raises(ValueError):
