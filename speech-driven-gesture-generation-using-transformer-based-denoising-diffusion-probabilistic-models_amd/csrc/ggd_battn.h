@@ -41,6 +41,7 @@ struct BtArgs : ggd_tr_battn_args {
   int group;       // query heads of a kv head
   int off;         // offset, clamped (past the table's distance on either side all is one bucket)
   int splits;      // parts of the streamed axis (few, dq, dkv)
+  int fine;        // bf16: weights and ds go into their products with the rest of their rounding too
   int vec_o;       // the written rows take 4-element stores
   int64_t hq, hk;  // elements between the heads of a row of q and dout, of k and v (dk, or what it is padded to)
   int64_t lddo;    // elements between rows of dout
@@ -257,6 +258,18 @@ __device__ __forceinline__ void mma_cols(f32x16 (&acc)[DK / 32], const uint4* im
         }
       }
   }
+}
+
+// what mma_cols' rounding to bf16 leaves of p: a second product of it carries p to 16 bits (BtArgs::fine)
+__device__ __forceinline__ f32x16 unrounded(const f32x16& p) {
+  f32x16 x;
+#pragma unroll
+  for (int r = 0; r < 16; r += 2) {
+    const uint32_t w = pk_bf16(p[r], p[r + 1]);
+    x[r] = p[r] - __uint_as_float(w << 16);
+    x[r + 1] = p[r + 1] - __uint_as_float(w & 0xFFFF0000u);
+  }
+  return x;
 }
 
 __device__ __forceinline__ f32x16 zero16() {

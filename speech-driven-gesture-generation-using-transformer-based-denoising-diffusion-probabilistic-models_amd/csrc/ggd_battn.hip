@@ -63,6 +63,13 @@ bool few_rows(const BtArgs& a) {
   return rows <= 32 || (blocks < 128 && a.lk >= 512 && a.lk >= 4 * a.lq);
 }
 
+// bf16 weights and ds, rounded once for their products, are off by up to 2^-9 each: a result's own rounding again, and over few
+// keys more in dq, where the roundings of o's weights do not average out in delta = do . o.  Where the call is small, or reads
+// its keys for few rows, a second product of what the rounding left costs next to nothing.
+bool fine_weights(const BtArgs& a) {
+  return a.dtype == GGD_TR_BF16 && (few_rows(a) || a.lk <= 64 || (int64_t)a.n * a.heads * a.lq <= (1 << 22) / a.lk);
+}
+
 // Parts of a streamed axis of `tiles` tiles: the fewest whose rounds of blocks over the chip's `slots` take (nearly) the least time,
 // each part with at least `least` tiles, at most 64 of them.
 int parts(int64_t blocks, int64_t tiles, int64_t least, int64_t slots) {
@@ -174,6 +181,7 @@ int ggd_tr_battn_fwd(const ggd_tr_battn_args* args, void* stream) {
   a.vec_o = a.dk % 4 == 0 && a.ldo % 4 == 0 && a.bo % 4 == 0 && aligned(a.o, 4 * esize(a)) && aligned(a.o32, 16);
   const bool few = few_rows(a);
   a.splits = fwd_splits(a);
+  a.fine = fine_weights(a);
   a.part = (float*)((char*)a.ws + space.pack);
   const hipStream_t s = (hipStream_t)stream;
   if (rows(a, false, s) != hipSuccess) return -3;
@@ -193,6 +201,7 @@ int ggd_tr_battn_bwd(const ggd_tr_battn_args* args, void* stream) {
   a.rest = (float*)(at + space.delta + space.table);
   a.part = (float*)(at + space.delta + space.table + space.rest);
   a.vec_o = a.dk % 4 == 0 && aligned(a.dq, 4 * esize(a)) && aligned(a.dk_out, 4 * esize(a)) && aligned(a.dv, 4 * esize(a));
+  a.fine = fine_weights(a);
   const int dqs = dq_splits(a), dkvs = dkv_splits(a);
   const hipStream_t s = (hipStream_t)stream;
   if (rows(a, true, s) != hipSuccess) return -3;

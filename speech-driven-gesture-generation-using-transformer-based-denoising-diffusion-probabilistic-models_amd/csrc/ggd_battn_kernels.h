@@ -93,6 +93,7 @@ __device__ __forceinline__ void attend(Softmax<DK>& sm, const uint4* kimg, const
       for (int r = 0; r < 16; ++r) sm.l += s[b][r];
     }
     mma_cols<T, DK, true>(sm.o, vimg, 32 * b, s[b], &sm.lr);
+    if (sizeof(T) == 2 && a.fine) mma_cols<T, DK, true>(sm.o, vimg, 32 * b, unrounded(s[b]), &sm.lr);
   }
 }
 
@@ -261,6 +262,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1)
         if constexpr (sizeof(T) == 2) sm.l += s[e];
       }
       mma_cols<T, DK, true>(sm.o, vimg, 0, s, &sm.lr);
+      if (sizeof(T) == 2) mma_cols<T, DK, true>(sm.o, vimg, 0, unrounded(s), &sm.lr);   // (the few rows' rule is one of BtArgs::fine)
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -549,6 +551,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
         }
       }
       mma_cols<T, DK>(acc, kimg, 32 * b, dp);
+      if (sizeof(T) == 2 && a.fine) mma_cols<T, DK>(acc, kimg, 32 * b, unrounded(dp));
     }
   }
   if (i < a.lq) {
@@ -778,6 +781,10 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1)
       }
       mma_cols<T, DK>(dv, oimg, 32 * b, s);
       mma_cols<T, DK>(dk, qimg, 32 * b, dp);
+      if (sizeof(T) == 2 && a.fine) {
+        mma_cols<T, DK>(dv, oimg, 32 * b, unrounded(s));
+        mma_cols<T, DK>(dk, qimg, 32 * b, unrounded(dp));
+      }
     }
     }
     put(stats + (buf ^ 1) * 3 * QT);

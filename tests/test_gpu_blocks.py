@@ -430,6 +430,37 @@ def test_the_widest_heads_with_the_longest_distance(pkg, dtype):
     check_attention(pkg, ins, do, 2, 1, buckets=buckets, offset=-3)
 
 
+@pytest.mark.parametrize("relative", [False, True])
+@pytest.mark.parametrize("lk", [2, 5, 33, 64])
+def test_gradients_of_peaked_rows_over_few_keys(pkg, lk, relative):
+    """Rows whose weight lies on one key: ds are differences of nearly equal numbers there, and have to come from a delta
+    without bf16's roundings.  What is left is half a step (2^-8) of each ds in its product and of the result, and f32's
+    share: a score is off by (dk + 8) 2^-23 of the sum of its terms' sizes, exp by some steps, and dp like a score."""
+    n, lq, heads, dk = 2, 70, 2, 64
+    ins, do, _ = attention_inputs("bf16", n, lq, lk, heads, heads, dk, seed=lk, n_buckets=8 if relative else 0)
+    ins[0] = (ins[0] * 4).bfloat16()
+    buckets = pkg.RelativeBuckets(8, 16) if relative else None
+    got = run_attention(pkg, ins, do, heads, heads, buckets=buckets)
+    Q, K, V, dO = (heads_of(x, heads) for x in (*ins[:3], do))
+    s, size = Q @ K.transpose(-1, -2) / 8, Q.abs() @ K.abs().transpose(-1, -2) / 8
+    if relative:
+        b = ins[3].cpu().double().t()[:, bucket_line(buckets, lq, lk, 0)][None]
+        s, size = s + b, size + b.abs()
+    p, dp = s.softmax(-1), dO @ V.transpose(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    off_p = ((dk + 8) * 2.0 ** -23 * size + 2.0 ** -21).amax(-1, keepdim=True)
+    off_dp = (dk + 8) * 2.0 ** -23 * (dO.abs() @ V.abs().transpose(-1, -2)).amax(-1, keepdim=True)
+    off = 2.0 ** -8 * ds.abs() + p * 2 * (off_dp + off_p * dp.abs().amax(-1, keepdim=True))
+    for name, a, want, err in (("dq", got[1], ds @ K / 8, off @ K.abs() / 8),
+                               ("dk", got[2], ds.transpose(-1, -2) @ Q / 8, off.transpose(-1, -2) @ Q.abs() / 8)):
+        err = 1.01 * err + 2.0 ** -8 * (want.abs() + err)
+        close(a, rows_of(want), rows_of(err), name)
+    if relative:   # in f32: off without the rounding of ds
+        which = th.nn.functional.one_hot(bucket_line(buckets, lq, lk, 0), 8).double()
+        off = p * 2 * (off_dp + off_p * dp.abs().amax(-1, keepdim=True)) + n * (lq + lk) * 2.0 ** -24 * ds.abs()
+        close(got[4], th.einsum("nhij,ijb->bh", ds, which), th.einsum("nhij,ijb->bh", off, which), "dtable")
+
+
 def test_attention_leaves_other_memory_alone(pkg):
     """Outputs lie in fresh tensors: inputs stay as they are, and so does what lies around a view's rows."""
     ins, do, g = attention_inputs("bf16", 2, 33, 45, 2, 1, 24)
