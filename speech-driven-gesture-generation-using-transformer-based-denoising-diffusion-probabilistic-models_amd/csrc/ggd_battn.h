@@ -40,7 +40,7 @@ constexpr float BT_LOG2E = 1.4426950408889634f;
 struct BtArgs : ggd_tr_battn_args {
   int group;       // query heads of a kv head
   int off;         // offset, clamped (past the table's distance on either side all is one bucket)
-  int splits;      // parts of the streamed axis (few, dq, dkv)
+  int splits;      // parts of the streamed axis
   int fine;        // bf16: weights and ds go into their products with the rest of their rounding too
   int vec_o;       // the written rows take 4-element stores
   int64_t hq, hk;  // elements between the heads of a row of q and dout, of k and v (dk, or what it is padded to)
@@ -210,7 +210,7 @@ __device__ __forceinline__ void mma_rows(f32x16& acc, const uint4* img, int r0, 
 }
 
 // acc[mb] += (columns 32 mb .. + 31 of image rows r0 .. r0 + 31)^T times p, p as an acc of those rows.
-// bf16: p is rounded to bf16 here (half a step, 2^-9 of each weight, on sums that stay in f32); k slot 8 h + i
+// bf16: p is rounded to bf16 here (half a step, up to 2^-8 of each weight, on sums that stay in f32); k slot 8 h + i
 // of step s is row 16 s + 8 (i / 4) + 4 h + i % 4 -- the rows the half's registers hold -- read by two
 // transposing loads.  f32: k slot h of step (g, j) is row 8 g + 4 h + j.
 // sum (SUM): + this half's weights as they go into the product, after their rounding

@@ -98,7 +98,13 @@ __device__ __forceinline__ void attend(Softmax<DK>& sm, const uint4* kimg, const
 }
 
 // ---------------------------------------------------------------------------------------------
-// forward, many rows: a block per 128 query rows of one head; the waves share the key tiles
+// forward, many rows: a block per 128 query rows of one head; the waves share the key tiles.  32 rows a wave fill the
+// MFMA's N, and a tile of 64 keys in LDS (two: the next one arrives by LDS loads meanwhile) serves 4 of them.  Where blocks are
+// few the keys are divided too, and bt_join_kernel joins the parts.
+//   Bound by the VALU and the MFMA units, which two waves a SIMD overlap in part: exp, maximum and sum of a score are 4 VALU
+// operations a lane, and at dk = 64 take more time than its products (counters: VALU 70 %, MFMA 30 % of the cycles; no bank
+// conflict).  bf16, 8 clips x 16 heads, 4096 rows over 2048 keys, dk 128: 615 us, 670 TFLOP/s; 4 x 16 heads, 4096 over 4096, dk 64
+// with a bias: 409 us, 670.  f32, 4 x 8 heads, 600 over 1501, dk 64: 83 + 7 us in 3 parts, 67 TFLOP/s.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int DK, bool BIAS>
 __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) bt_fwd_kernel(BtArgs a) {
@@ -176,7 +182,8 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
 // forward, few rows: the rows of all heads of a kv head together, 32 a block; the block's waves take every
 // fourth tile of 32 keys each, blocks a part of the keys (splits), and the parts are joined by their
 // maxima and sums.  Bound by reading the keys and values once: a wave has its next tile in flight
-// while it works on one, and needs no barrier for it.
+// while it works on one, and needs no barrier for it.  bf16, 8 clips x 32 heads on 8 kv heads, one row over 32773 keys,
+// dk 128: 161 + 5 us, 5.0 TB/s; 32 clips x 8 heads over 1200, dk 64, with a bias: 20 + 4 us, 4.0 TB/s.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ int64_t few_prow(const BtArgs& a, int64_t pair, int tiles, int tile) { return (pair * tiles + tile) * 32; }
 
@@ -354,6 +361,9 @@ __global__ void __launch_bounds__(256) bt_join_kernel(BtArgs a) {
 // Weights stay without their row's 1 / l until the end: it is one factor of the lane's row.
 //   Table: ds go into a histogram over clamped distances, a copy a wave (diag_add); blocks past the table's distance
 // are summed in registers.
+//   Three products a score and one exp: bound by the MFMA and LDS reads that feed it (each 32 keys' image is read twice, by
+// rows and transposed).  The forward kernel's sizes: 716 us, 860 TFLOP/s at dk 128; 670 us, 615 at dk 64 with the table's
+// gradient; f32 118 + 7 us, 70.
 // ---------------------------------------------------------------------------------------------
 // the block's histogram copies and its lanes' sums past the distance -> a row of dtab.  first: the block's first query
 __device__ __forceinline__ void write_buckets(const BtArgs& a, float* hist, float past, float behind, int first, int64_t row) {
@@ -583,6 +593,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
 // f32 sum of many.  ds sum to zero over a row, so that what they do sum to is e_i, and each ds has p_ij e_i too
 // much: this kernel takes sum_i p_ij e_i off each distance's sum.  Only the places within the table's distance
 // are formed again (scores alone); the weights past it were summed on the way, and those behind are the remainder to 1.
+// 81 us of 4 x 16 heads, 4096 x 4096, distance 128, whose dq takes 670; 35 of 58 at 6 x 12 heads, 777 x 777, distance 200.
 template <typename T, int DK>
 __global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
   constexpr int KT = tile_rows<T, DK>(), IMG = KT * Img<T, DK>::UPR;
@@ -684,7 +695,10 @@ static __global__ void __launch_bounds__(64) bt_table_kernel(BtArgs a, int per, 
 
 // ---------------------------------------------------------------------------------------------
 // dk, dv: a block per 128 keys of a kv head; the queries of all its heads are streamed, head after head, so that
-// a shared head's gradient is one sum in registers
+// a shared head's gradient is one sum in registers.  Four products a score.  bf16 at dk 64 runs two waves a SIMD (4 x 16 heads,
+// 4096 x 4096: 725 us, 760 TFLOP/s); at 128 the two sums and the two stationary rows take 400 registers, one wave a SIMD is
+// left, and nothing overlaps its exp and LDS reads (8 clips x 4 kv heads of 4, 4096 x 2048: 1350 us, 610; the MFMA 28 % busy).
+// Two waves with the values in LDS instead spilled: 1590.  f32, 4 x 8 heads, 600 x 1501, dk 64: 168 us, 66 TFLOP/s.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int DK, bool BIAS>
 __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1) bt_dkv_kernel(BtArgs a) {

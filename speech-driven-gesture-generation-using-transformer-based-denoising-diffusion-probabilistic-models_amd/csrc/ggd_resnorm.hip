@@ -134,7 +134,8 @@ __device__ __forceinline__ void rn_stats(const float (&x)[NV * V], int d, int t,
   rs = 1.0f / sqrtf(q[0] / d + eps);
 }
 
-// One row a wave (TPR 64, 4 rows a block) or a block (TPR 256).
+// One row a wave (TPR 64, 4 rows a block) or a block (TPR 256).  Bound by HBM: bf16, 65536 rows of 1024: 112 us for four
+// tensors, 4.8 TB/s, the rate of a large copy.
 template <typename T, int V, int NV, int TPR>
 __global__ void __launch_bounds__(256) resnorm_fwd_kernel(RnFwd a) {
   __shared__ float red[8];
@@ -193,7 +194,8 @@ __global__ void __launch_bounds__(256) resnorm_fwd_kernel(RnFwd a) {
 // Backward of a segment of rows that share a gate row.  h' is formed again in f32 from h, y and the
 // gate (h itself is read in the place of the stored h', whose rounding would go into the f32 weight
 // gradients), the column sums stay in registers over the segment and leave as one row of partial
-// sums a block, which resnorm_sum_kernel adds in a fixed order.
+// sums a block, which resnorm_sum_kernel adds in a fixed order.  Bound by HBM: bf16, 16 clips of 4096 rows of 1024, gate by
+// clip: 191 us for six tensors, 4.2 TB/s, and 11 us of column sums.
 template <typename T, int V, int NV, int TPR>
 __global__ void __launch_bounds__(256) resnorm_bwd_kernel(RnBwd a) {
   __shared__ float red[8];
