@@ -107,7 +107,7 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) {
 }
 
 // One tile of rows from memory into an LDS image, straight (buffer loads to LDS: no registers, nothing for the VALU).
-// Thread t of instruction i fills unit t + i THREADS of the image, and reads the row's unit that swz puts there.  Rows whose
+// Thread t of 256 (a block's, or its half's) fills unit t + 256 i of the image in instruction i, and reads the row's unit that swz puts there.  Rows whose
 // bit is clear are not read: their offset lies past the buffer's end, and zeros go into the image.
 //   The loads are issued by asm (the builtin makes the compiler wait for them at the next LDS access); they have
 // landed after tile_ready().
@@ -119,7 +119,7 @@ struct Tile {
   int row;          // of instruction 0
   int off[KINDS];   // byte offset of its unit, BT_OUT past dk
   __device__ __forceinline__ void start(int64_t ld, int dk) {
-    const int t = threadIdx.x;
+    const int t = threadIdx.x & 255;
     row = t / UPR;
 #pragma unroll
     for (int k = 0; k < KINDS; ++k) {
@@ -129,7 +129,7 @@ struct Tile {
   }
   __device__ __forceinline__ void load(const T* base, int64_t ld, uint64_t bits, const uint4* img) const {
     const i32x4 rs = buffer_at(base);
-    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(img) + (threadIdx.x >> 6) * 1024);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(img) + ((threadIdx.x & 255) >> 6) * 1024);
     const int step = (int)(STEP * ld * (int64_t)sizeof(T));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -145,6 +145,9 @@ struct Tile {
 
 // the block's loads have landed in LDS, and every wave is past its last reads of the other buffer
 __device__ __forceinline__ void tile_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// the block's LDS writes are there for all of it; loads may still be under way
+__device__ __forceinline__ void lds_ready() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // the same through registers, for a wave alone (bt_few_kernel): the loads stay in flight while it works
 template <typename T, int DK, int ROWS, int THREADS>

@@ -25,9 +25,9 @@ int prepare(const ggd_tr_battn_args* in, BtArgs& a) {
     return -2;
   if (!a.table) a.distance = 0, a.n_buckets = 0;
   a.group = a.heads / a.kv_heads;
-  if ((int64_t)a.group * a.lq > INT32_MAX - 64 || (int64_t)a.n * a.heads > 1 << 23 || (int64_t)a.heads * a.n_buckets > 1 << 25 ||
-      (int64_t)a.n * a.heads * ((std::max(a.lq, a.lk) + 31) / 32) > 1 << 23)
-    return -2;   // rows of a kv head; threads of a launch (256 a block, 64 a table entry; an axis is divided only where there are few blocks)
+  if ((int64_t)a.group * a.lq > INT32_MAX - 64 || (int64_t)a.n * a.heads > 1 << 22 || (int64_t)a.heads * a.n_buckets > 1 << 25 ||
+      (int64_t)a.n * a.heads * ((std::max(a.lq, a.lk) + 31) / 32) > 1 << 22)
+    return -2;   // rows of a kv head; threads of a launch (up to 512 a block, 64 a table entry; an axis is divided only where there are few blocks)
   a.off = (int)std::max<int64_t>(-(1 << 30), std::min<int64_t>(1 << 30, a.offset));
   a.c = a.scale * BT_LOG2E;
   a.splits = 1;

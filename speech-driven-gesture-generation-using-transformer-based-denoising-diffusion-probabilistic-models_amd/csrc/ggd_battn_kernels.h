@@ -1,5 +1,7 @@
 // ggd_battn_kernels.h -- the kernels of ggd_battn.h for one element type (included by ggd_battn*.hip)
 #pragma once
+#include <type_traits>
+
 #include "ggd_battn.h"
 
 namespace ggd {
@@ -696,9 +698,7 @@ static __global__ void __launch_bounds__(64) bt_table_kernel(BtArgs a, int per, 
 // ---------------------------------------------------------------------------------------------
 // dk, dv: a block per 128 keys of a kv head; the queries of all its heads are streamed, head after head, so that
 // a shared head's gradient is one sum in registers.  Four products a score.  bf16 at dk 64 runs two waves a SIMD (4 x 16 heads,
-// 4096 x 4096: 725 us, 760 TFLOP/s); at 128 the two sums and the two stationary rows take 400 registers, one wave a SIMD is
-// left, and nothing overlaps its exp and LDS reads (8 clips x 4 kv heads of 4, 4096 x 2048: 1350 us, 610; the MFMA 28 % busy).
-// Two waves with the values in LDS instead spilled: 1590.  f32, 4 x 8 heads, 600 x 1501, dk 64: 168 us, 66 TFLOP/s.
+// 4096 x 4096: 725 us, 760 TFLOP/s); past 64 it has a kernel of its own below.  f32, 4 x 8 heads, 600 x 1501, dk 64: 168 us, 66 TFLOP/s.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int DK, bool BIAS>
 __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1) bt_dkv_kernel(BtArgs a) {
@@ -817,6 +817,161 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1)
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// dk, dv of bf16 heads past 64: two sums and two stationary rows are 400 registers, and one wave a SIMD overlaps nothing with its
+// products (1350 us at 8 clips x 4 kv heads of 4, 4096 x 2048, dk 128, padded; the MFMA 28 % busy).  So two waves share 32 keys: the first holds k and dv,
+// forms the weights, p^T do and hands the weights on in f32 through LDS; the second, 32 queries behind, holds v and dk, forms
+// dp, ds and ds^T q.  Each has two of the four products, and a SIMD two waves.  A tile is in use for one and a half rounds: three
+// buffers.  1206 us, 680 TFLOP/s; what is left are the barrier after each 32 queries and the VALU work beside the products.
+// ---------------------------------------------------------------------------------------------
+template <bool BIAS>
+__global__ void __launch_bounds__(512, 2) bt_dkv_pair_kernel(BtArgs a) {
+  typedef bf16_t T;
+  constexpr int DK = 128, QT = tile_rows<T, DK>(), IMG = QT * Img<T, DK>::UPR;
+  static_assert(QT == 64, "two blocks of 32 queries a tile");
+  extern __shared__ uint4 lds[];
+  // [3][q, do images], [4 pairs][2 blocks][4][64 lanes] weights, [3][3][QT] statistics (maximum, 1 / sum, delta), the bias line
+  f32x4* weights = (f32x4*)(lds + 6 * IMG);
+  float *stats = (float*)(weights + 4 * 2 * 4 * 64), *mem = stats + 9 * QT, *line = mem + a.distance + LINE_PAD;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t tiles = (a.lk + BT_ROWS - 1) / BT_ROWS, items = a.n * a.kv_heads * a.splits * tiles, w = work_item(items, a.splits * tiles);
+  if (w >= items) return;
+  const int key0 = (int)(w % tiles) * BT_ROWS, row0 = key0 + (wave & 3) * 32, j = row0 + (lane & 31), split = w / tiles % a.splits;
+  const int pair = w / tiles / a.splits, kvh = pair % a.kv_heads, D = a.distance;
+  const int64_t clip = pair / a.kv_heads;
+  const uint8_t* mask = a.mask ? a.mask + clip * a.bmask : nullptr;
+  const bool any = __ballot(mask_byte(mask, key0, 64, a.lk)) | __ballot(mask_byte(mask, key0 + 64, 64, a.lk));
+  const bool there = j < a.lk && (!mask || mask[j]);
+  const bool live = __ballot(there);
+  auto work = [&](auto which) {   // (the two ways apart, so that each has its registers to itself)
+    constexpr bool second = decltype(which)::value;
+    Frag<T, DK> own;   // k, v
+    const int64_t ld = second ? a.ldv : a.ldk;
+    own.load_rows((second ? (const T*)a.v + clip * a.bv : (const T*)a.k + clip * a.bk) + (int64_t)row0 * ld + (int64_t)kvh * a.hk, ld, a.dk, there);
+    f32x16 acc[DK / 32];   // dv, dk
+#pragma unroll
+    for (int mb = 0; mb < DK / 32; ++mb) acc[mb] = zero16();
+    const int qt = (a.lq + QT - 1) / QT, steps = a.group * qt, per = (steps + a.splits - 1) / a.splits;
+    const int s0 = any ? split * per : 0, s1 = any ? min(steps, s0 + per) : 0;
+    const uint8_t* q_mask = a.q_mask ? a.q_mask + clip * a.bq_mask : nullptr;
+    Tile<T, DK, QT> rows;   // the first waves load q, the second do
+    const int64_t ldr = second ? a.lddo : a.ldq;
+    rows.start(ldr, a.dk);
+    float st_m = 0.f, st_r = 0.f, st_d = 0.f;
+    auto load = [&](int step, uint64_t bits, int buf) {
+      const int head = kvh * a.group + step / qt, i0 = step % qt * QT;
+      const T* from = second ? (const T*)a.dout + clip * a.lq * a.lddo : (const T*)a.q + clip * a.bq;
+      rows.load(from + (int64_t)i0 * ldr + (int64_t)head * a.hq, ldr, bits, lds + (2 * buf + second) * IMG);
+      if (!second && tid < QT) {
+        const int64_t at = (clip * a.heads + head) * a.lq + i0 + tid;
+        const bool row = (bits >> tid) & 1;
+        st_m = row ? a.stat[2 * at] : INFINITY;
+        st_r = row ? a.stat[2 * at + 1] : 0.f;
+        st_d = row ? a.delta[at] : 0.f;
+      }
+    };
+    auto put = [&](int buf) {
+      float* sts = stats + buf * 3 * QT;
+      if (!second && tid < QT) {
+        sts[tid] = st_m;
+        sts[QT + tid] = st_r;
+        sts[2 * QT + tid] = st_d;
+      }
+    };
+    auto bytes = [&](int step) { return step < s1 ? mask_byte(q_mask, step % qt * QT, QT, a.lq) : 0; };
+    // queries 32 b .. of tile t, whose bits are bits: the first wave's half, and the second's
+    auto first_half = [&](int t, int buf, int b, uint64_t bits) {
+      if (!(uint32_t)(bits >> (32 * b))) return;
+      const uint4 *qimg = lds + buf * 2 * IMG, *oimg = qimg + IMG;
+      const float* sts = stats + buf * 3 * QT;
+      f32x16 s = zero16();
+      mma_rows<T, DK>(s, qimg, 32 * b, own);
+      if constexpr (BIAS) {
+        const int q0 = t % qt * QT + 32 * b + a.off;   // position of the block's first query
+        add_bias<-1>(s, line, a.c, j - (q0 + 4 * h), D, row0 - (q0 + 31), row0 + 31 - q0);
+      }
+      f32x4* out = weights + ((wave & 3) * 2 + b) * 4 * 64 + lane;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = 32 * b + 8 * g + 4 * h;
+        const f32x4 m = *(const f32x4*)(sts + at), rl = *(const f32x4*)(sts + QT + at);
+        f32x4 p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          p[e] = s[r] = __builtin_amdgcn_exp2f(BIAS ? s[r] - m[e] : fmaf(s[r], a.c, -m[e])) * rl[e];
+        }
+        out[64 * g] = p;
+      }
+      mma_cols<T, DK>(acc, oimg, 32 * b, s);
+      if (a.fine) mma_cols<T, DK>(acc, oimg, 32 * b, unrounded(s));
+    };
+    auto second_half = [&](int buf, int b, uint64_t bits) {
+      if (!(uint32_t)(bits >> (32 * b))) return;
+      const uint4 *qimg = lds + buf * 2 * IMG, *oimg = qimg + IMG;
+      const float* sts = stats + buf * 3 * QT + 2 * QT;
+      f32x16 dp = zero16();
+      mma_rows<T, DK>(dp, oimg, 32 * b, own);
+      const f32x4* in = weights + ((wave & 3) * 2 + b) * 4 * 64 + lane;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 p = in[64 * g], dl = *(const f32x4*)(sts + 32 * b + 8 * g + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * g + e] = p[e] * (dp[4 * g + e] - dl[e]);
+      }
+      mma_cols<T, DK>(acc, qimg, 32 * b, dp);
+      if (a.fine) mma_cols<T, DK>(acc, qimg, 32 * b, unrounded(dp));
+    };
+    uint64_t next = __ballot(bytes(s0)), before = 0;   // bits of the next tile and of the last
+    if (s0 < s1) {
+      load(s0, next, 0);
+      put(0);
+    }
+    int nb = bytes(s0 + 1), lined = -1, buf = 0, last = 0;
+    for (int t = s0; t < s1; ++t) {
+      const int to = buf == 2 ? 0 : buf + 1;
+      if constexpr (BIAS) {
+        if (t / qt != lined) {   // another head: its line, once all have done with the last one's
+          lds_ready();
+          lined = t / qt;
+          bias_line(mem, a, kvh * a.group + lined);
+        }
+      }
+      tile_ready();
+      const uint64_t bits = next;
+      next = __ballot(nb);
+      if (t + 1 < s1) load(t + 1, next, to);
+      nb = bytes(t + 2);
+      if (live) {
+        if constexpr (second) second_half(last, 1, before);
+        else first_half(t, buf, 0, bits);
+      }
+      lds_ready();
+      if (live) {
+        if constexpr (second) second_half(buf, 0, bits);
+        else first_half(t, buf, 1, bits);
+      }
+      put(to);
+      before = bits;
+      last = buf;
+      buf = to;
+    }
+    lds_ready();
+    if constexpr (second)
+      if (live) second_half(last, 1, before);
+    if (j >= a.lk) return;
+    if (!there)
+#pragma unroll
+      for (int mb = 0; mb < DK / 32; ++mb) acc[mb] = zero16();
+    const int64_t row = ((clip * a.lk + j) * a.kv_heads + kvh) * a.dk, all = (int64_t)a.n * a.lk * a.kv_heads * a.dk;
+    const float scale = second ? a.scale : 1.f;
+    if (a.splits == 1) store_row<T, DK>((T*)(second ? a.dk_out : a.dv) + row, acc, scale, a.dk, a.vec_o);
+    else store_row<float, DK>(a.part + (second ? split : a.splits + split) * all + row, acc, scale, a.dk, a.vec_o);
+  };
+  if (wave < 4) work(std::false_type{});
+  else work(std::true_type{});
+}
+
 // rows of heads that are not whole aligned 16-byte units, laid out anew as such: (clips rows heads) dkp elements, zeros past dk
 template <typename T>
 __global__ void __launch_bounds__(256) bt_pack_kernel(int64_t n, int rows, int heads, int dk, int dkp, const T* __restrict__ src, int64_t ld,
@@ -911,10 +1066,16 @@ struct Kernels {
   }
   static hipError_t dkv(const BtArgs& a, hipStream_t s) {
     static std::atomic<bool> done[64];
-    const size_t lds = IMAGES + 6 * KT * sizeof(float) + lines(a);
-    if (const hipError_t e = allow_lds(bt_dkv_kernel<T, DK, BIAS>, lds, done)) return e;
-    const uint32_t each = (a.lk + BT_ROWS - 1) / BT_ROWS * a.splits;
-    hipLaunchKernelGGL((bt_dkv_kernel<T, DK, BIAS>), dim3(work_grid(a.n * a.kv_heads * each, each)), dim3(256), lds, s, a);
+    const uint32_t each = (a.lk + BT_ROWS - 1) / BT_ROWS * a.splits, grid = work_grid(a.n * a.kv_heads * each, each);
+    if constexpr (sizeof(T) == 2 && DK == 128) {
+      const size_t lds = IMAGES / 2 * 3 + 4 * 2 * 4 * 64 * sizeof(f32x4) + 9 * KT * sizeof(float) + lines(a);
+      if (const hipError_t e = allow_lds(bt_dkv_pair_kernel<BIAS>, lds, done)) return e;
+      hipLaunchKernelGGL((bt_dkv_pair_kernel<BIAS>), dim3(grid), dim3(512), lds, s, a);
+    } else {
+      const size_t lds = IMAGES + 6 * KT * sizeof(float) + lines(a);
+      if (const hipError_t e = allow_lds(bt_dkv_kernel<T, DK, BIAS>, lds, done)) return e;
+      hipLaunchKernelGGL((bt_dkv_kernel<T, DK, BIAS>), dim3(grid), dim3(256), lds, s, a);
+    }
     if (const hipError_t e = hipGetLastError()) return e;
     if (a.splits == 1) return hipSuccess;
     const int64_t all = (int64_t)a.n * a.lk * a.kv_heads * a.dk;
