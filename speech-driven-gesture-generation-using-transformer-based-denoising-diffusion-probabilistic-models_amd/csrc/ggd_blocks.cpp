@@ -5,6 +5,7 @@
 // over 64 clips of 40 frames took 143 us of which its kernels are 34.  The entries come as addresses from native.py, so that
 // they are those of the library it loaded.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -88,6 +89,13 @@ void check_capture(const char* what, std::initializer_list<Tensor> inputs) {
   }
 }
 
+// The kernels know no tangents: one of an input's (or, in a backward pass, of an incoming gradient's) would be lost without an error.
+void check_tangents(const char* what, at::ArrayRef<Tensor> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 // Gradients come once: where a graph of them is asked for, one that raises when it is used.
 variable_list once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -159,6 +167,7 @@ struct Attention : torch::autograd::Function<Attention> {
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_tangents("attention backward", grads);
     const variable_list saved = ctx->get_saved_variables();
     const Inputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], ctx->saved_data["heads"].toInt(),
                     ctx->saved_data["kv_heads"].toInt(), ctx->saved_data["offset"].toInt(), ctx->saved_data["scale"].toDouble()};
@@ -200,6 +209,7 @@ Tensor mask_rows(const char* what, const char* name, const OptTensor& m, int64_t
 
 Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tensor& v, int64_t heads, std::optional<int64_t> kv, std::optional<double> sc,
                  const OptTensor& mask, const OptTensor& q_mask, const OptTensor& buckets, const OptTensor& table, int64_t offset) {
+  check_tangents(what, {q, k, v, or_none(table)});
   on_gpu(what, q);
   beside(what, "k", k, q), beside(what, "v", v, q), beside(what, "mask", mask, q), beside(what, "q_mask", q_mask, q), beside(what, "table", table, q);
   const int64_t kv_heads = kv.value_or(heads);
@@ -257,6 +267,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_tangents("residual_norm backward", grads);
     const variable_list saved = ctx->get_saved_variables();
     auto whole = [&](const char* name) { return ctx->saved_data[name].toInt(); };
     const int64_t rows = whole("rows"), d = whole("d"), gate_rows = whole("gate_rows"), kind = whole("kind");
@@ -310,6 +321,7 @@ int64_t gate_rows_of(const char* what, Tensor& gate, const Tensor& h) {
 std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre_g, const OptTensor& pre_b, const OptTensor& post_g, const OptTensor& post_b,
                                         const OptTensor& gate_in, double scale, int64_t kind, double eps) {
   const char* what = "residual_norm";
+  check_tangents(what, {h, y, or_none(gate_in), or_none(pre_g), or_none(pre_b), or_none(post_g), or_none(post_b)});
   on_gpu(what, h);
   if (!pre_g || (!post_g && post_b)) refuse(what, "a norm needs a weight");
   beside(what, "y", y, h), beside(what, "gate", gate_in, h);

@@ -151,3 +151,23 @@ def test_residual_norm_entry_refusals(native):
 def test_entries_are_declared(native):
     for name in ("ggd_tr_resnorm_fwd", "ggd_tr_resnorm_bwd", "ggd_tr_resnorm_ws", "ggd_tr_battn_fwd", "ggd_tr_battn_bwd", "ggd_tr_battn_ws"):
         assert name in native.EXPORTS
+
+
+def test_forward_mode_derivatives_are_refused(pkg):
+    """A tangent would be lost: NotImplementedError, whichever operand carries it, with reverse-mode gradients or without."""
+    fw = th.autograd.forward_ad
+    x, w, table = th.ones(1, 2, 8), th.ones(8), th.zeros(8, 2)
+    buckets = pkg.RelativeBuckets(8, 16, device="cpu")
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, th.ones_like(t))
+        for call in (lambda: pkg.cross_attention(dual(x), x, x, 2), lambda: pkg.cross_attention(x, dual(x), x, 2), lambda: pkg.cross_attention(x, x, dual(x), 2),
+                     lambda: pkg.cross_attention(dual(x.clone().requires_grad_()), x, x, 2),
+                     lambda: pkg.relative_attention(x, x, x, 2, buckets, dual(table)),
+                     lambda: pkg.residual_norm(dual(x), x, (w, None)), lambda: pkg.residual_norm(x, dual(x), (w, None)),
+                     lambda: pkg.residual_norm(x, x, (dual(w), None)), lambda: pkg.residual_norm(x, x, (w, dual(w))),
+                     lambda: pkg.residual_norm(x, x, (w, None), post=(dual(w), None)), lambda: pkg.residual_norm(x, x, (w, None), post=(w, dual(w))),
+                     lambda: pkg.residual_norm(x, x, (w, None), gate=dual(w))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with th.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

@@ -753,3 +753,19 @@ def test_refusals(pkg):
     (g,) = th.autograd.grad(cross(x, k, k, 4, kv_heads=2).sum(), [x], create_graph=True)
     with pytest.raises(RuntimeError):
         th.autograd.grad(g.sum(), [x])
+
+
+def test_forward_mode_derivatives_are_refused(pkg):
+    """... of the inputs, and of the gradients that come into a backward pass (forward over reverse)."""
+    fw = th.autograd.forward_ad
+    x, w = th.randn(2, 5, 16, device="cuda", requires_grad=True), th.ones(16, device="cuda")
+    for call in (lambda t: pkg.cross_attention(t, t, t, 2), lambda t: pkg.residual_norm(t, t, (w, None))[1]):
+        with fw.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(fw.make_dual(x.detach(), th.ones_like(x)))
+            o = call(x)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                th.autograd.grad(o, [x], fw.make_dual(th.ones_like(o), th.ones_like(o)))
+            (plain,) = th.autograd.grad(call(x), [x], th.ones_like(o))   # without a tangent all is as before
+        (want,) = th.autograd.grad(call(x), [x], th.ones_like(o))
+        assert th.equal(plain, want)
