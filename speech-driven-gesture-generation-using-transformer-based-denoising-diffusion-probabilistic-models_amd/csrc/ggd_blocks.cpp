@@ -7,10 +7,12 @@
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -87,6 +89,17 @@ void check_capture(const char* what, std::initializer_list<Tensor> inputs) {
     if (hipStreamIsCapturing(stream.stream(), &status) == hipSuccess && status == hipStreamCaptureStatusActive)
       refuse(what, "captured while an eager graph of an input is alive; let go of that graph's outputs first");
   }
+}
+
+// A tracer sees the allocation of an output and not the kernels that fill it, and a tensor that only stands for another has no memory
+// to give them.
+void check_traced(const char* what, at::ArrayRef<Tensor> inputs) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  bool traced = torch::jit::tracer::isTracing() || Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL) ||
+                c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+  for (const Tensor& t : inputs) traced = traced || (t.defined() && t.unsafeGetTensorImpl()->is_python_dispatch());
+  TORCH_CHECK_NOT_IMPLEMENTED(!traced, what, " cannot be traced, nor called with fake tensors");
 }
 
 // The kernels know no tangents: one of an input's (or, in a backward pass, of an incoming gradient's) would be lost without an error.
@@ -167,6 +180,7 @@ struct Attention : torch::autograd::Function<Attention> {
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_traced("attention backward", grads);
     check_tangents("attention backward", grads);
     const variable_list saved = ctx->get_saved_variables();
     const Inputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], ctx->saved_data["heads"].toInt(),
@@ -209,6 +223,7 @@ Tensor mask_rows(const char* what, const char* name, const OptTensor& m, int64_t
 
 Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tensor& v, int64_t heads, std::optional<int64_t> kv, std::optional<double> sc,
                  const OptTensor& mask, const OptTensor& q_mask, const OptTensor& buckets, const OptTensor& table, int64_t offset) {
+  check_traced(what, {q, k, v, or_none(mask), or_none(q_mask), or_none(table)});
   check_tangents(what, {q, k, v, or_none(table)});
   on_gpu(what, q);
   beside(what, "k", k, q), beside(what, "v", v, q), beside(what, "mask", mask, q), beside(what, "q_mask", q_mask, q), beside(what, "table", table, q);
@@ -267,6 +282,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_traced("residual_norm backward", grads);
     check_tangents("residual_norm backward", grads);
     const variable_list saved = ctx->get_saved_variables();
     auto whole = [&](const char* name) { return ctx->saved_data[name].toInt(); };
@@ -321,6 +337,7 @@ int64_t gate_rows_of(const char* what, Tensor& gate, const Tensor& h) {
 std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre_g, const OptTensor& pre_b, const OptTensor& post_g, const OptTensor& post_b,
                                         const OptTensor& gate_in, double scale, int64_t kind, double eps) {
   const char* what = "residual_norm";
+  check_traced(what, {h, y, or_none(gate_in), or_none(pre_g), or_none(pre_b), or_none(post_g), or_none(post_b)});
   check_tangents(what, {h, y, or_none(gate_in), or_none(pre_g), or_none(pre_b), or_none(post_g), or_none(post_b)});
   on_gpu(what, h);
   if (!pre_g || (!post_g && post_b)) refuse(what, "a norm needs a weight");

@@ -171,3 +171,27 @@ def test_forward_mode_derivatives_are_refused(pkg):
                 call()
             with th.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_tracing_is_refused(pkg):
+    """A trace would hold the outputs' allocations without the kernels: NotImplementedError under every tracer, and for
+    tensors without memory."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w = th.ones(1, 2, 8), th.ones(8)
+    table, buckets = th.zeros(8, 2), pkg.RelativeBuckets(8, 16, device="cpu")
+    for call in (lambda t: pkg.cross_attention(t, t, t, 2), lambda t: pkg.relative_attention(t, t, t, 2, buckets, table),
+                 lambda t: pkg.residual_norm(t, t, (w, None))[1]):
+        with pytest.raises(NotImplementedError, match="traced"):
+            th.jit.trace(call, (x,))
+        for mode in ("real", "fake", "symbolic"):
+            with pytest.raises(NotImplementedError, match="traced"):
+                make_fx(call, tracing_mode=mode)(x)
+        with pytest.raises(NotImplementedError, match="traced"):
+            make_fx(call, pre_dispatch=True)(x)
+        with FakeTensorMode() as mode:
+            fake = th.empty(1, 2, 8, device="cuda")
+            with pytest.raises(NotImplementedError, match="traced"):
+                call(fake)
+        with pytest.raises(NotImplementedError, match="traced"):
+            call(fake)

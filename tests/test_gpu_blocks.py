@@ -769,3 +769,27 @@ def test_forward_mode_derivatives_are_refused(pkg):
             (plain,) = th.autograd.grad(call(x), [x], th.ones_like(o))   # without a tangent all is as before
         (want,) = th.autograd.grad(call(x), [x], th.ones_like(o))
         assert th.equal(plain, want)
+
+
+def test_tracing_is_refused_and_counting_modes_are_not(pkg):
+    """Modes that only look at the operations torch runs leave a call as it is."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Count(TorchDispatchMode):
+        seen = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen += 1
+            return func(*args, **(kwargs or {}))
+
+    x, w = th.randn(2, 5, 16, device="cuda"), th.ones(16, device="cuda")
+    for call in (lambda t: pkg.cross_attention(t, t, t, 2), lambda t: pkg.residual_norm(t, t, (w, None))[1]):
+        want = call(x)
+        with pytest.raises(NotImplementedError, match="traced"):
+            th.jit.trace(call, (x,))
+        with pytest.raises(NotImplementedError, match="traced"):
+            make_fx(call)(x)
+        with Count() as mode:
+            got = call(x)
+        assert mode.seen and th.equal(got, want)
