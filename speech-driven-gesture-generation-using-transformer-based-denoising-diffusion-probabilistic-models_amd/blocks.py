@@ -95,7 +95,8 @@ def cross_attention(q, k, v, heads, kv_heads=None, scale=None, mask=None, q_mask
     others is not read, their gradients are zero, and so is a row that may attend nothing (or that is
     not there).  Returns (n, Lq, heads dk).  Any lengths from 0 on: few queries over a long memory -- a
     stream's newest frame -- divide the memory among the chip.
-    (clips x heads x (rows or keys / 32, rounded up) up to 2^22; past it ValueError.)
+    (clips x heads x (rows or keys / 32, rounded up) up to 2^22, and rows of heads x dk below 32.5 MiB; past it
+    ValueError.)
     """
     return _attention("cross_attention", q, k, v, heads, kv_heads, scale, mask, q_mask, None, None, 0)
 

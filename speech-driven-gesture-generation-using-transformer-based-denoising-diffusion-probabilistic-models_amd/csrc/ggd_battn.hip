@@ -23,6 +23,9 @@ int prepare(const ggd_tr_battn_args* in, BtArgs& a) {
   if (!a.table != !a.buckets || (a.table && (a.n_buckets < 1 || a.distance < 1))) return -1;
   if (a.dk > BT_MAX_DK || a.lq > BT_MAX_ROWS || a.lk > BT_MAX_ROWS || (a.table && (a.n_buckets > BT_MAX_BUCKETS || a.distance > BT_MAX_DISTANCE)))
     return -2;
+  // rows that are packed lie their own width apart, and a tile of 64 of them is read by 32-bit byte offsets
+  const int64_t head_bytes = (a.dk * (a.dtype == GGD_TR_F32 ? 4 : 2) + 15) / 16 * 16;
+  if (63 * a.heads * head_bytes + head_bytes > INT32_MAX) return -2;
   if (!a.table) a.distance = 0, a.n_buckets = 0;
   a.group = a.heads / a.kv_heads;
   if ((int64_t)a.group * a.lq > INT32_MAX - 64 || (int64_t)a.n * a.heads > 1 << 22 || (int64_t)a.heads * a.n_buckets > 1 << 25 ||
@@ -37,7 +40,8 @@ int prepare(const ggd_tr_battn_args* in, BtArgs& a) {
 size_t esize(const BtArgs& a) { return a.dtype == GGD_TR_F32 ? 4 : 2; }
 
 // The kernels read rows in 16-byte units, and a tile of 64 rows by 32-bit offsets: rows that do not start at a multiple of 16
-// bytes, hold other than whole units or lie too far apart are packed first (one more pass over them, without a limit on strides).
+// bytes, hold other than whole units or lie too far apart are packed first (one more pass over them, without a limit on strides;
+// prepare() has one on their width).
 constexpr int64_t BT_MAX_LD = 1 << 22;
 bool whole_rows(const BtArgs& a, const void* p, int64_t ld, int64_t b) {
   const int64_t per = 16 / (int64_t)esize(a);

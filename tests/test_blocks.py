@@ -195,3 +195,19 @@ def test_tracing_is_refused(pkg):
                 call(fake)
         with pytest.raises(NotImplementedError, match="traced"):
             call(fake)
+
+
+@pytest.mark.parametrize("dtype,heads,dk", [(1, 3 << 16, 128), (0, 3 << 15, 128), (0, 3 << 16, 64), (1, 3 << 19, 9), (0, 3 << 19, 5)])
+def test_rows_too_wide_for_their_offsets_are_unsupported(native, dtype, heads, dk):
+    """A tile has 64 rows, whose byte offsets are 32-bit numbers: 63 rows' width past 2^31 would wrap, and rows of another place or zeros be
+    read.  (The workspace is left out, so that an entry that takes the shape answers -1 and launches nothing.)"""
+    lib = native.load()
+    size = 4 if dtype == 0 else 2
+    width = heads * ((dk * size + 15) // 16 * 16)
+    assert 63 * width + 16 * ((dk * size + 15) // 16) > (1 << 31) - 1
+    for over, want in ((dict(heads=heads), -2), (dict(heads=heads // 2), -1)):
+        args = _battn(native, n=1, kv_heads=1, lq=64, lk=64, dk=dk, dtype=dtype, ldq=8, bq=8, ldk=8, bk=8, ldv=8, bv=8, ws=None, ws_bytes=0, **over)
+        assert lib.ggd_tr_battn_bwd(ctypes.byref(args), None) == want
+        args.ldq = 1 << 23   # packed
+        assert lib.ggd_tr_battn_fwd(ctypes.byref(args), None) == want
+        assert (lib.ggd_tr_battn_ws(ctypes.byref(args), 1) > 0) == (want == -1)
