@@ -137,9 +137,12 @@ struct Tile {
       issue(rs, (bits >> (row + i * STEP)) & 1 && o != BT_OUT ? o + i * step : BT_OUT, at + i * 4096);
     }
   }
-  // (five wait states: the descriptor and the address may come from the VALU's readfirstlane)
+  // (five wait states: the descriptor and the address may come from the VALU's readfirstlane.  m0 is given back: it is not a register
+  // that asm can declare as written)
   static __device__ __forceinline__ void issue(i32x4 rs, int offset, uint32_t at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(rs) : "memory");
+    uint32_t kept;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(kept) : "s"(at), "v"(offset), "s"(rs) : "memory");
   }
 };
 
