@@ -60,16 +60,21 @@ Packed packed_space(const BtArgs& a) {
   return {up((int64_t)a.n * a.lq * a.heads * row), up((int64_t)a.n * a.lk * a.kv_heads * row)};
 }
 
-// Few rows: the rows of a kv head's query heads fit one MFMA tile (32), or the tiled kernel's blocks of 128
-// rows of a head would leave most of the chip idle while the keys are long enough to divide among blocks.
+// Few rows: the rows of a kv head's query heads fit one MFMA tile (32), or the call is small beside the keys it reads and the tiled
+// kernel's blocks of 128 rows would not fill the chip.  Blocks of 32 rows start sooner and divide finer: bf16, 8 heads of 64,
+// 128 rows over 16384 keys 31 us for the tiled kernel's 50, f32, 2 heads, 256 over 4096 26 for 35.  Past 2^24 scores they read each
+// key too often: bf16, 8 heads of 128, 1000 rows over 16000 271 us for 90, f32, 2 heads of 64, 4000 over 16000 408 for 286; and f32
+// heads past 64, of one wave a SIMD, past 2^22: 8 heads of 128, 256 over 4096 128 us for 70.
 bool few_rows(const BtArgs& a) {
   const int64_t rows = (int64_t)a.group * a.lq, blocks = (int64_t)a.n * a.heads * ((a.lq + BT_ROWS - 1) / BT_ROWS);
-  return rows <= 32 || (blocks < 128 && a.lk >= 512 && a.lk >= 4 * a.lq);
+  const int64_t scores = a.dtype == GGD_TR_F32 && a.dk > 64 ? 1 << 22 : 1 << 24;
+  return rows <= 32 || (blocks < 128 && a.lk >= 512 && a.lk >= 4 * a.lq && (int64_t)a.n * a.heads * a.lq <= scores / a.lk);
 }
 
 // bf16 weights and ds, rounded once for their products, are off by up to 2^-8 each: a result's own rounding again, and over few
 // keys more in dq, where the roundings of o's weights do not average out in delta = do . o.  Where the call is small, or reads
-// its keys for few rows, a second product of what the rounding left costs next to nothing: 33 -> 37 us of a training pass's
+// its keys for few rows, a second product of what the rounding left costs little (few rows up to 32 are bound by their keys, more of them
+// up to 6 % of a training pass: 86 -> 91 us for 8 heads of 64, 256 rows over 8192): 33 -> 37 us of a training pass's
 // kernels at 2^21 scores (whose host side takes 65), 465 -> 493 at 256 clips x 8 heads, 500 over 64 keys; above it stays one, 100 -> 116 us
 // at 2^25 scores.
 bool fine_weights(const BtArgs& a) {

@@ -95,6 +95,17 @@ def test_many_rows_over_divided_keys(pkg, shape, dtype, relative):
     check_attention(pkg, ins, do, heads, kv_heads, buckets=buckets)
 
 
+# scores on both sides of 2^24, and of 2^22 for f32 heads past 64: the few rows' kernel gives way to blocks of 128 rows
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 800, 5200, 4, 2, 64), (1, 850, 5200, 4, 2, 64), (2, 140, 3700, 4, 4, 128), (2, 140, 3800, 4, 4, 128)], ids=str)
+def test_many_rows_over_far_more_keys(pkg, shape, dtype):
+    n, lq, lk, heads, kv_heads, dk = shape
+    assert lk >= 4 * lq and n * heads * ((lq + 127) // 128) < 128
+    ins, do, g = attention_inputs(dtype, *shape)
+    mask, q_mask = masks(n, lq, lk, g)
+    check_attention(pkg, ins, do, heads, kv_heads, mask=mask, q_mask=q_mask)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("lq,lk", [(1, 40), (40, 33), (130, 70)])
 def test_kv_heads_that_do_not_fill_the_xcds(pkg, lq, lk, dtype):
