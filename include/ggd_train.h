@@ -158,7 +158,8 @@ int64_t ggd_tr_resnorm_ws(int64_t rows, int d, int64_t gate_rows, int has_gate);
  * bias; heads of dk <= 128 elements, f32 or bf16 (sums and softmax in f32):
  *   s_ij = scale q_i . k_j + table[bucket(j - i - offset)][head],  o_i = sum_j softmax_j(s_ij) v_j
  * over the keys that mask allows; a row with none is zeros.  Query head h reads kv head h / (heads / kv_heads).
- * -2 past clips x heads x (rows or keys / 32) of 2^22, and where 63 rows of heads (each of whole 16-byte units) and a head pass 2^31 - 1 bytes.
+ * -2 past 2^28 rows or keys, clips x heads x (rows / 32) of 2^22, where a backward pass follows clips x kv_heads x
+ * (keys / 128) of 2^22, and where 63 rows of heads (each of whole 16-byte units) and a head pass 2^31 - 1 bytes.
  * Memory of masked keys and queries is not read: whatever it holds reaches nothing. */
 typedef struct ggd_tr_battn_args {
   int32_t n, heads, kv_heads, lq, lk, dk;  /* lq, lk >= 1 */

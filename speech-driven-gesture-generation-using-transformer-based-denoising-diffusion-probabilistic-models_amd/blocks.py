@@ -93,10 +93,10 @@ def cross_attention(q, k, v, heads, kv_heads=None, scale=None, mask=None, q_mask
     reads kv head h // (heads / kv_heads).  scale: 1 / sqrt(dk) by default, > 0.  mask (n, Lk) / q_mask
     (n, Lq), truth values: the states that may be attended, and the queries that are there; memory of the
     others is not read, their gradients are zero, and so is a row that may attend nothing (or that is
-    not there).  Returns (n, Lq, heads dk).  Any lengths from 0 on: few queries over a long memory -- a
+    not there).  Returns (n, Lq, heads dk).  Lengths from 0 on: few queries over a long memory -- a
     stream's newest frame -- divide the memory among the chip.
-    (clips x heads x (rows or keys / 32, rounded up) up to 2^22, and rows of heads x dk below 32.5 MiB; past it
-    ValueError.)
+    (Limits, past which there is a ValueError: 2^28 rows and states; clips x heads x (rows / 32, rounded up) up to 2^22; with
+    gradients clips x kv_heads x (states / 128, rounded up) up to 2^22; rows of heads x dk below 32.5 MiB.)
     """
     return _attention("cross_attention", q, k, v, heads, kv_heads, scale, mask, q_mask, None, None, 0)
 

@@ -13,7 +13,7 @@ constexpr int BT_MAX_ROWS = 1 << 28;   // rows and keys: positions and distances
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
 // 0, -1 (argument) or -2 (unsupported), and the launch-side fields
-int prepare(const ggd_tr_battn_args* in, BtArgs& a) {
+int prepare(const ggd_tr_battn_args* in, BtArgs& a, bool backward) {
   if (!in) return -1;
   (ggd_tr_battn_args&)a = *in;
   if (a.n < 0 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || a.lq < 1 || a.lk < 1 || a.dk < 1 ||
@@ -29,8 +29,10 @@ int prepare(const ggd_tr_battn_args* in, BtArgs& a) {
   if (!a.table) a.distance = 0, a.n_buckets = 0;
   a.group = a.heads / a.kv_heads;
   if ((int64_t)a.group * a.lq > INT32_MAX - 64 || (int64_t)a.n * a.heads > 1 << 22 || (int64_t)a.heads * a.n_buckets > 1 << 25 ||
-      (int64_t)a.n * a.heads * ((std::max(a.lq, a.lk) + 31) / 32) > 1 << 22)
-    return -2;   // rows of a kv head; threads of a launch (up to 512 a block, 64 a table entry; an axis is divided only where there are few blocks)
+      (int64_t)a.n * a.heads * ((a.lq + 31) / 32) > 1 << 22)
+    return -2;   // rows of a kv head; threads of a launch (256 a block, 64 a table entry; an axis is divided only where there are few blocks)
+  // ... and 512 a block of 128 keys in the backward pass, where one follows; the forward pass has no block a key
+  if ((backward || a.stat) && (int64_t)a.n * a.kv_heads * ((a.lk + BT_ROWS - 1) / BT_ROWS) > 1 << 22) return -2;
   a.off = (int)std::max<int64_t>(-(1 << 30), std::min<int64_t>(1 << 30, a.offset));
   a.c = a.scale * BT_LOG2E;
   a.splits = 1;
@@ -177,13 +179,13 @@ extern "C" {
 
 int64_t ggd_tr_battn_ws(const ggd_tr_battn_args* args, int backward) {
   BtArgs a{};
-  if (prepare(args, a) || a.n == 0) return 0;
+  if (prepare(args, a, backward) || a.n == 0) return 0;
   return (backward ? backward_space(a) : forward_space(a)).all();
 }
 
 int ggd_tr_battn_fwd(const ggd_tr_battn_args* args, void* stream) {
   BtArgs a{};
-  if (const int e = prepare(args, a)) return e;
+  if (const int e = prepare(args, a, false)) return e;
   if (a.n == 0) return 0;
   if (!a.q || !a.k || !a.v || !a.o || !a.stat != !a.o32) return -1;
   const Space space = forward_space(a);
@@ -201,7 +203,7 @@ int ggd_tr_battn_fwd(const ggd_tr_battn_args* args, void* stream) {
 
 int ggd_tr_battn_bwd(const ggd_tr_battn_args* args, void* stream) {
   BtArgs a{};
-  if (const int e = prepare(args, a)) return e;
+  if (const int e = prepare(args, a, true)) return e;
   if (a.n == 0) return 0;
   if (!a.q || !a.k || !a.v || !a.stat || !a.o32 || !a.dout || !a.dq || !a.dk_out || !a.dv || (a.dtable && !a.table)) return -1;
   const Space space = backward_space(a);

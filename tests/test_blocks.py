@@ -211,3 +211,16 @@ def test_rows_too_wide_for_their_offsets_are_unsupported(native, dtype, heads, d
         args.ldq = 1 << 23   # packed
         assert lib.ggd_tr_battn_fwd(ctypes.byref(args), None) == want
         assert (lib.ggd_tr_battn_ws(ctypes.byref(args), 1) > 0) == (want == -1)
+
+
+def test_long_memories_are_limited_by_the_launches_they_need(native):
+    """8 clips of 32 heads over 3 million states (17 hours at 50 a second): the forward pass has no block a key, the backward pass one of
+    128 keys a kv head.  (The workspace is left out: an entry that takes the shape answers -1 and launches nothing.)"""
+    lib = native.load()
+    shape = dict(n=8, heads=32, kv_heads=8, lq=1, dk=16, ldq=512, bq=512, ldk=128, ldv=128, bk=1 << 40, bv=1 << 40, ldo=512, bo=512, ws=None, ws_bytes=0)
+    for lk, stat, want in ((3000000, None, -1), (3000000, 1 << 20, -1), (1 << 28, None, -1), (1 << 23, 1 << 20, -1), ((1 << 23) + 1, 1 << 20, -2)):
+        args = _battn(native, lk=lk, stat=stat, o32=stat, **shape)
+        assert lib.ggd_tr_battn_fwd(ctypes.byref(args), None) == want, (lk, stat)
+        assert (lib.ggd_tr_battn_ws(ctypes.byref(args), 0) > 0) == (want == -1)
+        args = _battn(native, lk=lk, **shape)
+        assert lib.ggd_tr_battn_bwd(ctypes.byref(args), None) == (-1 if lk <= 1 << 23 else -2)

@@ -112,3 +112,25 @@ def test_kv_heads_that_do_not_fill_the_xcds(pkg, lq, lk, dtype):
     """66 clips' kv heads, dealt to 8 XCDs in turn: the last round has two."""
     ins, do, g = attention_inputs(dtype, 11, lq, lk, 12, 6, 32)
     check_attention(pkg, ins, do, 12, 6, mask=make_mask("holes", 11, lk, g))
+
+
+def test_many_heads_over_a_long_memory(pkg):
+    """512 heads on 16 kv heads over 270000 states.  Values grow along the memory, so that a part of it left out, or read twice, shows.
+    f32: a lane adds every eighth key of one of at least 32 parts one after another, 1055 at most, the parts follow: 1200 U
+    of o's terms twice (weights and their sum), and a weight's own error is 2 (dk + 8) U of its score's terms."""
+    heads, kv_heads, dk, lk = 512, 16, 8, 270000
+    assert heads * (lk // 32) > 1 << 22
+    g = th.Generator(device="cuda").manual_seed(1)
+    q, k = (th.randn(1, length, h * dk, generator=g, device="cuda") for length, h in ((1, heads), (lk, kv_heads)))
+    v = th.linspace(0, 1, lk, device="cuda")[None, :, None] + th.rand(1, lk, kv_heads * dk, generator=g, device="cuda")
+    with th.no_grad():
+        got = pkg.cross_attention(q, k, v, heads, kv_heads=kv_heads)
+    split = lambda x, h: x.double().reshape(-1, h, dk).transpose(0, 1).contiguous()
+    Q, K, V = split(q, heads).reshape(kv_heads, heads // kv_heads, dk), split(k, kv_heads), split(v, kv_heads)
+    for h in range(kv_heads):
+        s, size = Q[h] @ K[h].t() / math.sqrt(dk), Q[h].abs() @ K[h].abs().t() / math.sqrt(dk)
+        p = s.softmax(-1)
+        want = p @ V[h]
+        err = (2 * 1200 * U + 2 * (dk + 8) * U * size.amax(-1, keepdim=True)) * want + U * want
+        out = got.reshape(kv_heads, heads // kv_heads, dk)[h].double()
+        assert bool(((out - want).abs() <= err).all()), (h, (out - want).abs().max().item(), err.max().item())
