@@ -49,17 +49,18 @@ bool whole_rows(const BtArgs& a, const void* p, int64_t ld, int64_t b) {
   const int64_t per = 16 / (int64_t)esize(a);
   return aligned(p, 16) && ld % per == 0 && ld <= BT_MAX_LD && b % per == 0 && a.dk % per == 0;
 }
-bool packed(const BtArgs& a, bool backward) {
-  const int64_t ldo = (int64_t)a.heads * a.dk;
-  return !whole_rows(a, a.q, a.ldq, a.bq) || !whole_rows(a, a.k, a.ldk, a.bk) || !whole_rows(a, a.v, a.ldv, a.bv) ||
-         (backward && !whole_rows(a, a.dout, ldo, ldo));
-}
 int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-// bytes of packed q (and dout) and of packed k (and v)
-struct Packed { int64_t q, k; };
-Packed packed_space(const BtArgs& a) {
-  const int64_t per = 16 / (int64_t)esize(a), row = (a.dk + per - 1) / per * 16;
-  return {up((int64_t)a.n * a.lq * a.heads * row), up((int64_t)a.n * a.lk * a.kv_heads * row)};
+// bytes of each operand's packed rows, 0 where it is read in place: an operand out of line is packed alone (a stream's new query does not
+// copy its memory), but where dk itself is no whole units all are
+struct Packed {
+  int64_t q, k, v, dout;
+  int64_t all() const { return q + k + v + dout; }
+};
+Packed packed_space(const BtArgs& a, bool backward) {
+  const int64_t per = 16 / (int64_t)esize(a), row = (a.dk + per - 1) / per * 16, ldo = (int64_t)a.heads * a.dk;
+  const int64_t q = up((int64_t)a.n * a.lq * a.heads * row), k = up((int64_t)a.n * a.lk * a.kv_heads * row);
+  return {whole_rows(a, a.q, a.ldq, a.bq) ? 0 : q, whole_rows(a, a.k, a.ldk, a.bk) ? 0 : k, whole_rows(a, a.v, a.ldv, a.bv) ? 0 : k,
+          !backward || whole_rows(a, a.dout, ldo, ldo) ? 0 : q};
 }
 
 // Few rows: the rows of a kv head's query heads fit one MFMA tile (32), or the call is small beside the keys it reads and the tiled
@@ -122,8 +123,7 @@ struct Space {
 };
 Space backward_space(const BtArgs& a) {
   Space s;
-  const Packed p = packed_space(a);
-  s.pack = packed(a, true) ? 2 * (p.q + p.k) : 0;
+  s.pack = packed_space(a, true).all();
   s.delta = up((int64_t)a.n * a.heads * a.lq * 4);
   const int ds = dq_splits(a), ks = dkv_splits(a);
   const int two = a.dtype == GGD_TR_BF16;
@@ -136,8 +136,7 @@ Space backward_space(const BtArgs& a) {
 }
 Space forward_space(const BtArgs& a) {
   Space s{};
-  const Packed p = packed_space(a);
-  if (packed(a, false)) s.pack = p.q + 2 * p.k;
+  s.pack = packed_space(a, false).all();
   if (const int splits = fwd_splits(a); splits > 1)
     s.part = up(((int64_t)a.group * a.lq + 31) / 32 * 32 * a.n * a.kv_heads * splits * (dk_class(a) + 4) * 4);
   return s;
@@ -147,24 +146,23 @@ const Launch& launch(const BtArgs& a) { return a.dtype == GGD_TR_F32 ? battn_f32
 
 // q, k, v (and dout) as the kernels read them, packed into the workspace's first part where they have to be
 hipError_t rows(BtArgs& a, bool backward, hipStream_t s) {
-  a.hq = a.hk = a.dk;
-  a.lddo = (int64_t)a.heads * a.dk;
-  if (!packed(a, backward)) return hipSuccess;
-  const Packed p = packed_space(a);
+  const Packed p = packed_space(a, backward);
   const int64_t per = 16 / (int64_t)esize(a), dkp = (a.dk + per - 1) / per * per;
   char* at = (char*)a.ws;
   const Launch& l = launch(a);
-  if (const hipError_t e = l.pack(a, a.q, a.ldq, a.bq, a.lq, a.heads, at, s)) return e;
-  if (const hipError_t e = l.pack(a, a.k, a.ldk, a.bk, a.lk, a.kv_heads, at + p.q, s)) return e;
-  if (const hipError_t e = l.pack(a, a.v, a.ldv, a.bv, a.lk, a.kv_heads, at + p.q + p.k, s)) return e;
-  if (backward) {
-    if (const hipError_t e = l.pack(a, a.dout, a.lddo, a.lq * a.lddo, a.lq, a.heads, at + p.q + 2 * p.k, s)) return e;
-    a.dout = at + p.q + 2 * p.k;
-  }
-  a.q = at, a.k = at + p.q, a.v = at + p.q + p.k;
-  a.hq = a.hk = dkp;
-  a.ldq = a.lddo = a.heads * dkp, a.bq = a.lq * a.ldq;
-  a.ldk = a.ldv = a.kv_heads * dkp, a.bk = a.bv = a.lk * a.ldk;
+  auto pack = [&](int64_t bytes, const void*& src, int64_t& ld, int64_t& b, int rows, int heads) {
+    if (!bytes) return hipSuccess;
+    const hipError_t e = l.pack(a, src, ld, b, rows, heads, at, s);
+    src = at, ld = heads * dkp, b = rows * ld;
+    at += bytes;
+    return e;
+  };
+  int64_t bdo = a.lq * (a.lddo = (int64_t)a.heads * a.dk);
+  if (const hipError_t e = pack(p.q, a.q, a.ldq, a.bq, a.lq, a.heads)) return e;
+  if (const hipError_t e = pack(p.k, a.k, a.ldk, a.bk, a.lk, a.kv_heads)) return e;
+  if (const hipError_t e = pack(p.v, a.v, a.ldv, a.bv, a.lk, a.kv_heads)) return e;
+  if (const hipError_t e = pack(p.dout, a.dout, a.lddo, bdo, a.lq, a.heads)) return e;
+  a.hq = a.hk = dkp;   // (dk where one is read in place)
   return hipSuccess;
 }
 

@@ -224,3 +224,18 @@ def test_long_memories_are_limited_by_the_launches_they_need(native):
         assert (lib.ggd_tr_battn_ws(ctypes.byref(args), 0) > 0) == (want == -1)
         args = _battn(native, lk=lk, **shape)
         assert lib.ggd_tr_battn_bwd(ctypes.byref(args), None) == (-1 if lk <= 1 << 23 else -2)
+
+
+def test_an_operand_out_of_line_is_packed_alone(native):
+    """The workspace holds the rows that are laid out anew: of the one operand that is not in whole aligned 16-byte units."""
+    lib = native.load()
+    need = lambda backward, **over: lib.ggd_tr_battn_ws(ctypes.byref(_battn(native, **dict(dict(lk=300, bk=9600, bv=9600), **over))), backward)
+    at, q, k = 1 << 20, 2 * 3 * 4 * 16 * 2, 2 * 300 * 2 * 16 * 2   # bytes of q's rows and of k's
+    up = lambda x: (x + 255) // 256 * 256
+    for backward in (0, 1):
+        plain = need(backward)
+        for over, more in ((dict(q=at + 2), up(q)), (dict(ldq=68, bq=204), up(q)), (dict(k=at + 8), up(k)), (dict(v=at + 4, bv=9601), up(k)),
+                           (dict(q=at + 2, k=at + 2), up(q) + up(k)), (dict(dout=at + 6), up(q) if backward else 0)):
+            assert need(backward, **over) - plain == more, over
+        odd = dict(dk=15, ldq=60, ldk=30, ldv=30)
+        assert need(backward, **odd) >= (2 if backward else 1) * up(q) + 2 * up(k)

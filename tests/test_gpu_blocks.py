@@ -793,3 +793,30 @@ def test_tracing_is_refused_and_counting_modes_are_not(pkg):
         with Count() as mode:
             got = call(x)
         assert mode.seen and th.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk", [(3, 90), (140, 200)])
+def test_each_operand_out_of_line_alone(pkg, lq, lk, dtype):
+    """Rows one element past an aligned address, or an odd number of elements apart, beside others that are read in place."""
+    n, heads, kv_heads, dk = 2, 4, 2, 40
+    ins, do, _ = attention_inputs(dtype, n, lq, lk, heads, kv_heads, dk)
+    want = run_attention(pkg, ins, do, heads, kv_heads)
+    check_attention(pkg, ins, do, heads, kv_heads)
+
+    def off(x):
+        store = th.full((n, x.shape[1], x.shape[2] + 3), 9., dtype=x.dtype, device="cuda")
+        view = store[..., 1:-2]
+        view.copy_(x)
+        return view
+
+    for at in range(4):
+        xs = [off(x) if i == at else x for i, x in enumerate((*ins, do))]
+        leaves = [x.detach().requires_grad_() for x in xs[:3]]
+        o = pkg.cross_attention(*leaves, heads, kv_heads=kv_heads)
+        grad = xs[3]
+        if at == 3:   # a contiguous gradient off its alignment
+            grad = th.empty(do.numel() + 1, dtype=do.dtype, device="cuda")[1:].view(do.shape)
+            grad.copy_(do)
+        for a, b in zip([o, *th.autograd.grad(o, leaves, grad)], want):
+            assert th.equal(a, b), at
