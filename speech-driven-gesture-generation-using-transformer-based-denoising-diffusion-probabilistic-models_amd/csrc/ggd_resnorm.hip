@@ -37,6 +37,7 @@ struct RnBwd {
   void *dh, *dy, *dgate;
   float* part;  // [5][blocks][d]: pre weight, pre bias, post weight, post bias, gate sums of each block
   int64_t seg, segs;   // rows of a block, all of one gate row, and blocks of a gate row
+  int64_t per, groups; // per > 0: a block has `per` whole gate rows of the `groups` there are instead, and writes their sums itself
   int64_t group_rows;  // rows of a gate row (all rows without a gate, and where each row has its own)
   bool by_row;         // each row has its own gate row
 };
@@ -191,26 +192,36 @@ __global__ void __launch_bounds__(256) resnorm_fwd_kernel(RnFwd a) {
   }
 }
 
-// Backward of a segment of rows that share a gate row.  h' is formed again in f32 from h, y and the
-// gate (h itself is read in the place of the stored h', whose rounding would go into the f32 weight
-// gradients), the column sums stay in registers over the segment and leave as one row of partial
+// Backward of a segment of rows that share a gate row, or of several gate rows' rows (a wave has whole gate rows then).  h' is
+// formed again in f32 from h, y and the gate (h itself is read in the place of the stored h', whose rounding would go into the f32
+// weight gradients), the column sums stay in registers over the segment and leave as one row of partial
 // sums a block, which resnorm_sum_kernel adds in a fixed order.  Bound by HBM: bf16, 16 clips of 4096 rows of 1024, gate by
 // clip: 191 us for six tensors, 4.2 TB/s, and 11 us of column sums.
-template <typename T, int V, int NV, int TPR>
+template <typename T, int V, int NV, int TPR, bool SEVERAL>
 __global__ void __launch_bounds__(256) resnorm_bwd_kernel(RnBwd a) {
   __shared__ float red[8];
   __shared__ float colred[TPR == 64 ? 3 * 64 * NV * V : 1];
   constexpr int E = NV * V, WAVES = 256 / TPR;
   const RnFwd& f = a.f;
   const int t = threadIdx.x & (TPR - 1), wave = TPR == 64 ? threadIdx.x >> 6 : 0, d = f.d;
-  const int64_t group = blockIdx.x / a.segs, s0 = (blockIdx.x % a.segs) * a.seg;
-  const int64_t r0 = group * a.group_rows + s0, r1 = min(r0 + a.seg, (group + 1) * a.group_rows);
   float ng[E], pg[E], sng[E], snb[E], spg[E], spb[E], sgt[E];
   rn_load<float, V, NV, TPR>(ng, f.ng, d, t);
   if (f.pg) rn_load<float, V, NV, TPR>(pg, f.pg, d, t);
 #pragma unroll
   for (int e = 0; e < E; ++e) sng[e] = snb[e] = spg[e] = spb[e] = sgt[e] = 0.f;
-  for (int64_t row = r0 + wave; row < r1; row += WAVES) {
+  // a segment, its rows dealt to the waves; SEVERAL: the wave's own gate rows, one after another
+  int64_t row, end;
+  int left = f.gate_rows;   // rows to the end of the gate row
+  if constexpr (SEVERAL) {
+    const int64_t group = blockIdx.x * a.per + wave * (a.per / WAVES);
+    row = group * a.group_rows;
+    end = min(group + a.per / WAVES, a.groups) * a.group_rows;
+  } else {
+    const int64_t group = blockIdx.x / a.segs, r0 = group * a.group_rows + (blockIdx.x % a.segs) * a.seg;
+    row = r0 + wave;
+    end = min(r0 + a.seg, (group + 1) * a.group_rows);
+  }
+  for (; row < end; row += SEVERAL ? 1 : WAVES) {
     float h[E], y[E], dt[E], du[E], gt[E];
     rn_load<T, V, NV, TPR>(y, (const T*)f.y + row * d, d, t);
     rn_load<T, V, NV, TPR>(h, (const T*)f.h + row * d, d, t);
@@ -288,6 +299,12 @@ __global__ void __launch_bounds__(256) resnorm_bwd_kernel(RnBwd a) {
       for (int e = 0; e < E; ++e) dt[e] = rs1 * (dt[e] - n1 - y[e] * n2);
     }
     rn_store<T, V, NV, TPR>((T*)a.dy + row * d, dt, d, t);
+    if (SEVERAL && --left == 0) {
+      rn_store<T, V, NV, TPR>((T*)a.dgate + (int64_t)((uint32_t)row / (uint32_t)f.gate_rows) * d, sgt, d, t);
+      left = f.gate_rows;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sgt[e] = 0.f;
+    }
   }
   // the block's column sums: its waves' in order, then one row a kind
   const int64_t blocks = gridDim.x;
@@ -308,7 +325,7 @@ __global__ void __launch_bounds__(256) resnorm_bwd_kernel(RnBwd a) {
   if (f.nb) leave(snb, 1);
   if (f.pg) leave(spg, 2);
   if (f.pb) leave(spb, 3);
-  if (f.gate && !a.by_row) leave(sgt, 4);
+  if (f.gate && !a.by_row && !SEVERAL) leave(sgt, 4);
 }
 
 // Column sums of the partial rows: block (x, y) adds 64 columns of list y -- one of the weights'
@@ -356,32 +373,42 @@ int rn_check(const RnFwd& a, int dtype, int kind) {
   return a.d > RN_MAX_D || a.rows > RN_MAX_ROWS ? -2 : 0;
 }
 
-// blocks of the backward pass: segments of a gate row's rows, about 1024 blocks in all (4 a CU) but at
-// least 8 rows each, so that the partial sums stay a small part of the traffic
-struct RnSegments { int64_t group_rows, groups, seg, segs; };
-RnSegments rn_segments(int64_t rows, int64_t gate_rows, bool gate) {
-  RnSegments g;
+// Blocks of the backward pass: segments of a gate row's rows, about 1024 blocks in all (4 a CU) but at least 8 rows each, so that
+// the partial sums stay a small part of the traffic.  Where there are more gate rows than that (than waves of as many blocks, where
+// each wave has rows of its own), a block or wave has whole gate rows, several of them, in 1024 to 2048 blocks: bf16, a training pass
+// over 200000 gate rows of 2 rows of 64 columns 3054 -> 588 us against a block a gate row, 5000 of 20 rows of 1024 602 -> 524.
+struct RnSegments { int64_t group_rows, groups, seg, segs, per, blocks; };
+RnSegments rn_segments(int64_t rows, int d, int64_t gate_rows, bool gate) {
+  RnSegments g{};
   g.group_rows = gate && gate_rows > 1 ? gate_rows : rows;
   g.groups = rows / g.group_rows;
+  const int64_t waves = d <= 1024 ? 4 : 1;   // (RN_DISPATCH: a row a wave, or a block)
+  if (g.groups > 1024 * waves) {
+    g.per = (g.groups + 2048 * waves - 1) / (2048 * waves) * waves;
+    g.blocks = (g.groups + g.per - 1) / g.per;
+    return g;
+  }
   const int64_t want = std::max<int64_t>(1, 1024 / g.groups);
   g.seg = std::max<int64_t>(std::min<int64_t>(8, g.group_rows), (g.group_rows + want - 1) / want);
   g.segs = (g.group_rows + g.seg - 1) / g.seg;
+  g.blocks = g.segs * g.groups;
   return g;
 }
 
-#define RN_DISPATCH(KERNEL, T, VMAX, vec, d, GRID)                                                                   \
-  if (vec) {                                                                                                         \
-    if (d <= 256 * VMAX / 4) { GRID(64, (KERNEL<T, VMAX, 1, 64>)); }                                                 \
-    else if (d <= 512 * VMAX / 4 && d <= 1024) { GRID(64, (KERNEL<T, VMAX, 2, 64>)); }                               \
-    else if (d <= 1024) { GRID(64, (KERNEL<T, VMAX, 16 / VMAX, 64>)); }                                              \
-    else if (d <= 2048) { GRID(256, (KERNEL<T, VMAX, 8 / VMAX, 256>)); }                                             \
-    else if (d <= 4096) { GRID(256, (KERNEL<T, VMAX, 16 / VMAX, 256>)); }                                            \
-    else { GRID(256, (KERNEL<T, VMAX, 32 / VMAX, 256>)); }                                                           \
-  } else {                                                                                                           \
-    if (d <= 256) { GRID(64, (KERNEL<T, 1, 4, 64>)); }                                                               \
-    else if (d <= 1024) { GRID(64, (KERNEL<T, 1, 16, 64>)); }                                                        \
-    else if (d <= 4096) { GRID(256, (KERNEL<T, 1, 16, 256>)); }                                                      \
-    else { GRID(256, (KERNEL<T, 1, 32, 256>)); }                                                                     \
+// (further arguments: more of the kernel's template arguments, from their comma on)
+#define RN_DISPATCH(KERNEL, T, VMAX, vec, d, GRID, ...)                                            \
+  if (vec) {                                                                                       \
+    if (d <= 256 * VMAX / 4) { GRID(64, (KERNEL<T, VMAX, 1, 64 __VA_ARGS__>)); }                   \
+    else if (d <= 512 * VMAX / 4 && d <= 1024) { GRID(64, (KERNEL<T, VMAX, 2, 64 __VA_ARGS__>)); } \
+    else if (d <= 1024) { GRID(64, (KERNEL<T, VMAX, 16 / VMAX, 64 __VA_ARGS__>)); }                \
+    else if (d <= 2048) { GRID(256, (KERNEL<T, VMAX, 8 / VMAX, 256 __VA_ARGS__>)); }               \
+    else if (d <= 4096) { GRID(256, (KERNEL<T, VMAX, 16 / VMAX, 256 __VA_ARGS__>)); }              \
+    else { GRID(256, (KERNEL<T, VMAX, 32 / VMAX, 256 __VA_ARGS__>)); }                             \
+  } else {                                                                                         \
+    if (d <= 256) { GRID(64, (KERNEL<T, 1, 4, 64 __VA_ARGS__>)); }                                 \
+    else if (d <= 1024) { GRID(64, (KERNEL<T, 1, 16, 64 __VA_ARGS__>)); }                          \
+    else if (d <= 4096) { GRID(256, (KERNEL<T, 1, 16, 256 __VA_ARGS__>)); }                        \
+    else { GRID(256, (KERNEL<T, 1, 32, 256 __VA_ARGS__>)); }                                       \
   }
 
 }  // namespace
@@ -413,8 +440,7 @@ int ggd_tr_resnorm_fwd(int64_t rows, int d, int dtype, int kind, float scale, fl
 
 int64_t ggd_tr_resnorm_ws(int64_t rows, int d, int64_t gate_rows, int has_gate) {
   if (rows <= 0 || rows > RN_MAX_ROWS || d <= 0 || d > RN_MAX_D || gate_rows < 1 || (has_gate && rows % gate_rows)) return 0;
-  const RnSegments g = rn_segments(rows, gate_rows, has_gate);
-  return 5 * g.segs * g.groups * d * (int64_t)sizeof(float);
+  return 5 * rn_segments(rows, d, gate_rows, has_gate).blocks * d * (int64_t)sizeof(float);
 }
 
 int ggd_tr_resnorm_bwd(int64_t rows, int d, int dtype, int kind, float scale, float eps, const void* h, const void* y,
@@ -430,31 +456,31 @@ int ggd_tr_resnorm_bwd(int64_t rows, int d, int dtype, int kind, float scale, fl
       !post_b != !d_post_b)
     return -1;
   if (!ws || !rn_aligned(ws) || ws_bytes < ggd_tr_resnorm_ws(rows, d, gate_rows, gate != nullptr)) return -1;
-  const RnSegments g = rn_segments(rows, gate_rows, gate);
-  a.seg = g.seg, a.segs = g.segs, a.group_rows = g.group_rows;
+  const RnSegments g = rn_segments(rows, d, gate_rows, gate);
+  a.seg = g.seg, a.segs = g.segs, a.per = g.per, a.groups = g.groups, a.group_rows = g.group_rows;
   a.by_row = gate && gate_rows == 1;
-  const int64_t blocks = g.segs * g.groups;
-  if (blocks > RN_MAX_GRID) return -2;
   const bool vec = d % (dtype == GGD_TR_F32 ? 4 : 8) == 0 && rn_aligned(h) && rn_aligned(y) && rn_aligned(gate) && rn_aligned(post_g) &&
                    rn_aligned(post_b) && rn_aligned(pre_g) && rn_aligned(pre_b) && rn_aligned(dh_out) && rn_aligned(du) &&
                    rn_aligned(dh) && rn_aligned(dy) && rn_aligned(dgate);
   hipStream_t s = (hipStream_t)stream;
-#define RN_GRID(TPR, K) hipLaunchKernelGGL(K, dim3((unsigned)blocks), dim3(256), 0, s, a)
+#define RN_GRID(TPR, K) hipLaunchKernelGGL(K, dim3((unsigned)g.blocks), dim3(256), 0, s, a)
   if (dtype == GGD_TR_F32) {
-    RN_DISPATCH(resnorm_bwd_kernel, float, 4, vec, d, RN_GRID)
+    if (g.per) { RN_DISPATCH(resnorm_bwd_kernel, float, 4, vec, d, RN_GRID, , true) }
+    else { RN_DISPATCH(resnorm_bwd_kernel, float, 4, vec, d, RN_GRID, , false) }
   } else {
-    RN_DISPATCH(resnorm_bwd_kernel, bf16_t, 8, vec, d, RN_GRID)
+    if (g.per) { RN_DISPATCH(resnorm_bwd_kernel, bf16_t, 8, vec, d, RN_GRID, , true) }
+    else { RN_DISPATCH(resnorm_bwd_kernel, bf16_t, 8, vec, d, RN_GRID, , false) }
   }
 #undef RN_GRID
   RnSum r{};
-  r.d = d, r.blocks = blocks, r.segs = g.segs, r.part = a.part, r.dgate = dgate, r.bf16 = dtype == GGD_TR_BF16;
+  r.d = d, r.blocks = g.blocks, r.segs = g.segs, r.part = a.part, r.dgate = dgate, r.bf16 = dtype == GGD_TR_BF16;
   float* const out[4] = {d_pre_g, d_pre_b, d_post_g, d_post_b};
   for (int k = 0; k < 4; ++k)
     if (out[k]) {
       r.out[r.gate0] = out[k];
       r.kind[r.gate0++] = k;
     }
-  r.lists = r.gate0 + (gate && !a.by_row ? g.groups : 0);
+  r.lists = r.gate0 + (gate && !a.by_row && !g.per ? g.groups : 0);
   hipLaunchKernelGGL(resnorm_sum_kernel, dim3((d + 63) / 64, (unsigned)std::min<int64_t>(r.lists, 65535)), dim3(1024), 0, s, r);
   return hipGetLastError() == hipSuccess ? 0 : -3;
 }

@@ -239,3 +239,15 @@ def test_an_operand_out_of_line_is_packed_alone(native):
             assert need(backward, **over) - plain == more, over
         odd = dict(dk=15, ldq=60, ldk=30, ldv=30)
         assert need(backward, **odd) >= (2 if backward else 1) * up(q) + 2 * up(k)
+
+
+def test_partial_sums_of_many_gate_rows_stay_few(native):
+    """Blocks of the backward pass, and with them the partial sums, are bounded whatever the number of gate rows, each of 2 to 7 rows; a count
+    past any limit of a launch is no other case."""
+    lib = native.load()
+    for d in (64, 1024, 1032, 8192):
+        for groups in (1, 1000, 1025, 4097, 100000, (1 << 22) + 1, (1 << 28)):
+            for rows in (2, 7):
+                blocks = lib.ggd_tr_resnorm_ws(groups * rows, d, rows, 1) / (5 * d * 4)
+                assert 0 < blocks <= 4096, (d, groups, rows, blocks)
+        assert lib.ggd_tr_resnorm_ws(1 << 30, d, 1, 0) / (5 * d * 4) <= 1024

@@ -820,3 +820,36 @@ def test_each_operand_out_of_line_alone(pkg, lq, lk, dtype):
             grad.copy_(do)
         for a, b in zip([o, *th.autograd.grad(o, leaves, grad)], want):
             assert th.equal(a, b), at
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind,post", [("layer", True), ("rms", False)])
+@pytest.mark.parametrize("shape", [(4500, 2, 64), (20000, 2, 64), (9000, 3, 37), (5000, 7, 130), (1100, 2, 1032), (2500, 3, 1029), (4400, 2, 1000)], ids=str)
+def test_residual_norm_with_many_gate_rows(pkg, shape, dtype, kind, post):
+    """More gate rows than blocks: waves, and past 1024 columns blocks, have whole gate rows, several of them."""
+    h, y, pre, post, G = norm_inputs(dtype, shape, "clip", kind, post)
+    check_norm(pkg, h, y, pre, post, G, 0.9, kind)
+
+
+def test_residual_norm_with_millions_of_gate_rows(pkg):
+    """2^22 + 3 gate rows of 2 rows: what belongs to a row or gate row has the bits of the two halves' calls, whose gradients of the
+    weights add up (to n U of the sums of sizes)."""
+    n, d = (1 << 22) + 3, 8
+    g = th.Generator(device="cuda").manual_seed(2)
+    rnd = lambda *s: th.randn(*s, generator=g, device="cuda")
+    h, y, gate, dh, du = rnd(n, 2, d), rnd(n, 2, d), rnd(n, 1, d), rnd(n, 2, d), rnd(n, 2, d)
+    w = [1 + 0.1 * rnd(d) for _ in range(4)]
+
+    def call(at):
+        leaves = [t.detach().requires_grad_() for t in (h[at], y[at], gate[at], *w)]
+        out = pkg.residual_norm(leaves[0], leaves[1], leaves[3:5], post=leaves[5:7], gate=leaves[2], scale=0.5)
+        return [o.detach() for o in out] + list(th.autograd.grad(out, leaves, (dh[at], du[at])))
+
+    whole, one, two = call(slice(None)), call(slice(0, n // 2)), call(slice(n // 2, n))
+    for a, b, c in zip(whole[:5], one, two):
+        assert th.equal(a, th.cat([b, c]))
+    # a block adds at most 2 (n / 1024 / 4 + 1) rows a wave one after another, 4 waves, then 2048 / 16 blocks and 16 lists; each term is
+    # below 8 * 8 * 3 (a gradient of 8, a norm of sqrt(8) < 3 and a gate below 8, twice over)
+    steps = 2 * (n // 4096 + 1) + 4 + 2048 // 16 + 16
+    for a, b, c in zip(whole[5:], one[5:], two[5:]):
+        assert bool(((a - (b + c)).abs() <= 2 * steps * U * 2 * n * 8).all())
