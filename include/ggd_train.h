@@ -134,7 +134,7 @@ int ggd_tr_head_flatten(int N, int H, int W, int C, const float* src, float* dst
 
 /* ---- operators of a decoder block beyond the reference's (…_amd/blocks.py) ---- */
 enum { GGD_TR_F32 = 0, GGD_TR_BF16 = 1 };             /* dtype of the row tensors; weights and statistics are f32 */
-enum { GGD_TR_LAYERNORM = 0, GGD_TR_RMSNORM = 1 };    /* kind */
+enum { GGD_TR_LAYERNORM = 0, GGD_TR_RMSNORM = 1, GGD_TR_GATE_F32 = 16 };    /* kind; GATE_F32: added, see ggd_tr_gate_sum */
 
 /* The norms around a block with its gate and residual scale, over contiguous rows of d <= 8192:
  *   h_out = scale h + gate * post(y),  u = pre(h_out before its rounding)
@@ -153,6 +153,13 @@ int ggd_tr_resnorm_bwd(int64_t rows, int d, int dtype, int kind, float scale, fl
                        void* dgate, float* d_post_g, float* d_post_b, float* d_pre_g, float* d_pre_b, void* ws,
                        int64_t ws_bytes, void* stream);
 int64_t ggd_tr_resnorm_ws(int64_t rows, int d, int64_t gate_rows, int has_gate);
+/* A gate that is broadcast along other axes than whole trailing rows is expanded to one row a row (gate_rows 1); its gradient is
+ * left in f32, [rows][d], where the backward pass's kind has GGD_TR_GATE_F32 added, and summed by this: out (dtype, contiguous over the
+ * kept axes) = sums of src (f32, contiguous, `axes` sizes of 1 or more) over the axes whose kept is 0, in f32 and a fixed order.
+ * ws: ggd_tr_gate_sum_ws(...) bytes.  More than 8 runs of kept or of summed axes in turn are -2. */
+int ggd_tr_gate_sum(int axes, const int64_t* sizes, const uint8_t* kept, const float* src, int dtype, void* out, void* ws,
+                    int64_t ws_bytes, void* stream);
+int64_t ggd_tr_gate_sum_ws(int axes, const int64_t* sizes, const uint8_t* kept);
 
 /* Attention for any lengths, with masks, kv heads shared by query heads, and a learned relative position
  * bias; heads of dk <= 128 elements, f32 or bf16 (sums and softmax in f32):

@@ -132,7 +132,8 @@ def residual_norm(h, y, pre, post=None, gate=None, scale=1.0, kind="layer", eps=
     h (the residual stream) and y (the block's output): (..., d) of one shape and type, float32 or bfloat16,
     d <= 8192.  pre and post are (weight, bias) of a norm over d, in float32, bias or the whole of post
     None: LayerNorm (kind "layer") or RMS norm (kind "rms").  gate: of h's type, broadcast to h -- (d,),
-    one row a clip (n, 1, d), one a token -- or None.  u is the norm of h' before h' is rounded to its
+    one row a clip (n, 1, d), one a token -- or None; another shape that broadcasts (one row a frame, one element a
+    token) is expanded to h's, and its gradient summed in f32.  u is the norm of h' before h' is rounded to its
     type.  Gradients reach h, y, gate and the weights.
     """
     what = "residual_norm"

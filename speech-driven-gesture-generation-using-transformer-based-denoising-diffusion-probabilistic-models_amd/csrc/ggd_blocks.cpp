@@ -38,6 +38,8 @@ struct Entries {
   decltype(&ggd_tr_resnorm_fwd) resnorm_fwd;
   decltype(&ggd_tr_resnorm_bwd) resnorm_bwd;
   decltype(&ggd_tr_resnorm_ws) resnorm_ws;
+  decltype(&ggd_tr_gate_sum) gate_sum;
+  decltype(&ggd_tr_gate_sum_ws) gate_sum_ws;
 } entries;
 
 // ValueError of what does not hold
@@ -255,7 +257,23 @@ Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tenso
 struct Shape {
   int64_t rows, d, gate_rows, kind;
   double scale, eps;
+  bool expanded;   // the gate is read expanded to h's shape
 };
+
+// the gate as the kernels read it
+Tensor whole_gate(const Tensor& gate, const Tensor& h, bool expanded) { return expanded ? gate.expand(h.sizes()).contiguous() : gate; }
+
+// an expanded gate's gradient, of h's shape in f32, -> that of the gate
+void sum_gate(const Tensor& whole, const Tensor& gate, Tensor& out) {
+  const int64_t dims = whole.dim(), less = dims - gate.dim();
+  c10::SmallVector<uint8_t, 8> kept;
+  for (int64_t i = 0; i < dims; ++i) kept.push_back(i >= less && gate.size(i - less) == whole.size(i));
+  const int64_t bytes = entries.gate_sum_ws((int)dims, whole.sizes().data(), kept.data());
+  const Tensor ws = workspace(bytes, whole);
+  const int rc = entries.gate_sum((int)dims, whole.sizes().data(), kept.data(), at_of<const float>(whole), dtype_of(out), at_of(out), at_of(ws), bytes,
+                                  stream_of(whole));
+  TORCH_CHECK(rc == 0, "residual_norm backward failed (ggd_train status ", rc, ")");
+}
 
 variable_list norm_forward(const Tensor& h, const Tensor& y, const Tensor& gate, const variable_list& w, const Shape& g, bool keep, Tensor& stats) {
   Tensor h_out = at::empty_like(h), u = at::empty_like(h);
@@ -272,11 +290,13 @@ variable_list norm_forward(const Tensor& h, const Tensor& y, const Tensor& gate,
 
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& y, const OptTensor& gate, const OptTensor& post_g,
-                               const OptTensor& post_b, const OptTensor& pre_g, const OptTensor& pre_b, int64_t rows, int64_t d, int64_t gate_rows, int64_t kind, double scale, double eps) {
+                               const OptTensor& post_b, const OptTensor& pre_g, const OptTensor& pre_b, int64_t rows, int64_t d, int64_t gate_rows, int64_t kind, double scale, double eps,
+                               bool expanded) {
     Tensor stats;
     const variable_list w{or_none(post_g), or_none(post_b), or_none(pre_g), or_none(pre_b)};
-    variable_list out = norm_forward(h, y, or_none(gate), w, {rows, d, gate_rows, kind, scale, eps}, true, stats);
-    ctx->save_for_backward({h, y, or_none(gate), w[0], w[1], w[2], w[3], stats});
+    const Tensor whole = whole_gate(or_none(gate), h, expanded);
+    variable_list out = norm_forward(h, y, whole, w, {rows, d, gate_rows, kind, scale, eps, expanded}, true, stats);
+    ctx->save_for_backward({h, y, or_none(gate), w[0], w[1], w[2], w[3], stats, expanded ? whole : Tensor()});
     ctx->saved_data["rows"] = rows, ctx->saved_data["d"] = d, ctx->saved_data["gate_rows"] = gate_rows, ctx->saved_data["kind"] = kind;
     ctx->saved_data["scale"] = scale, ctx->saved_data["eps"] = eps;
     return out;
@@ -288,12 +308,13 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     auto whole = [&](const char* name) { return ctx->saved_data[name].toInt(); };
     const int64_t rows = whole("rows"), d = whole("d"), gate_rows = whole("gate_rows"), kind = whole("kind");
     const float scale = (float)ctx->saved_data["scale"].toDouble(), eps = (float)ctx->saved_data["eps"].toDouble();
-    variable_list out(13);
+    variable_list out(14);
     {
       const at::NoGradGuard no_grad;
-      const Tensor &h = saved[0], &y = saved[1], &gate = saved[2], &stats = saved[7];
+      const bool expanded = saved[8].defined();
+      const Tensor &h = saved[0], &y = saved[1], &gate = expanded ? saved[8] : saved[2], &stats = saved[7];
       for (int i = 0; i < 7; ++i)
-        if (saved[i].defined()) out[i] = at::empty_like(saved[i]);
+        if (saved[i].defined()) out[i] = at::empty(saved[i].sizes(), saved[i].options());
       if (rows == 0) {
         for (Tensor& t : out)
           if (t.defined()) t.zero_();
@@ -302,19 +323,21 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor dh_out = grads[0].contiguous(), du = grads[1].contiguous();
         const int64_t bytes = entries.resnorm_ws(rows, (int)d, gate_rows, gate.defined());
         const Tensor ws = workspace(bytes, h);
-        const int rc = entries.resnorm_bwd(rows, (int)d, dtype_of(h), (int)kind, scale, eps, at_of(h), at_of(y), at_of(gate), gate_rows, at_of<float>(saved[3]),
+        const Tensor dgate = expanded ? at::empty(h.sizes(), h.options().dtype(at::kFloat)) : out[2];
+        const int rc = entries.resnorm_bwd(rows, (int)d, dtype_of(h), (int)kind | (expanded ? GGD_TR_GATE_F32 : 0), scale, eps, at_of(h), at_of(y), at_of(gate), gate_rows, at_of<float>(saved[3]),
                                            at_of<float>(saved[4]), at_of<float>(saved[5]), at_of<float>(saved[6]), at_of<float>(stats), at_of(dh_out),
-                                           at_of(du), at_of(out[0]), at_of(out[1]), at_of(out[2]), at_of<float>(out[3]), at_of<float>(out[4]),
+                                           at_of(du), at_of(out[0]), at_of(out[1]), at_of(dgate), at_of<float>(out[3]), at_of<float>(out[4]),
                                            at_of<float>(out[5]), at_of<float>(out[6]), at_of(ws), bytes, stream_of(h));
         TORCH_CHECK(rc == 0, "residual_norm backward failed (ggd_train status ", rc, ")");
+        if (expanded) sum_gate(dgate, saved[2], out[2]);
       }
     }
     return once(std::move(out), "residual_norm");
   }
 };
 
-// Rows of h that share a row of the gate; the gate as it is read: leading dimensions of h, then ones, then d.  Any other shape
-// that broadcasts is expanded.
+// Rows of h that share a row of the gate, which is read as it is: leading dimensions of h, then ones, then d.  Any other shape
+// that broadcasts is read expanded (0).
 int64_t gate_rows_of(const char* what, Tensor& gate, const Tensor& h) {
   const int64_t dims = h.dim(), less = dims - gate.dim();
   bool fits = gate.dim() >= 1 && less >= 0;
@@ -325,10 +348,7 @@ int64_t gate_rows_of(const char* what, Tensor& gate, const Tensor& h) {
   while (ones > 0 && size(ones - 1) == 1) --ones;
   bool direct = size(dims - 1) == h.size(dims - 1);
   for (int64_t i = 0; i < ones; ++i) direct = direct && size(i) == h.size(i);
-  if (!direct) {
-    gate = gate.expand(h.sizes()).contiguous();
-    return 1;
-  }
+  if (!direct) return 0;
   for (int64_t i = ones; i < dims - 1; ++i) shared *= h.size(i);
   gate = gate.contiguous();
   return std::max<int64_t>(1, shared);
@@ -358,24 +378,30 @@ std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre
       t = t.contiguous();
     }
   if (!std::isfinite((float)scale) || !std::isfinite((float)eps) || !((float)eps > 0.f)) refuse(what, "scale ", scale, " has to be finite, eps ", eps, " positive");
-  Shape g{h.numel() / d, d, 1, kind, scale, eps};
+  Shape g{h.numel() / d, d, 1, kind, scale, eps, false};
   Tensor gate = or_none(gate_in);
-  if (gate.defined()) g.gate_rows = gate_rows_of(what, gate, h);
+  if (gate.defined()) {
+    g.gate_rows = gate_rows_of(what, gate, h);
+    g.expanded = g.gate_rows == 0;
+    if (g.expanded && h.dim() > 16) refuse(what, "a gate along other axes than whole trailing rows has to have at most 16");
+    g.gate_rows = std::max<int64_t>(1, g.gate_rows);
+  }
   h = h.contiguous(), y = y.contiguous();
   variable_list out;
   if (grad && at::GradMode::is_enabled()) {
-    out = ResidualNorm::apply(h, y, given(gate), given(w[0]), given(w[1]), given(w[2]), given(w[3]), g.rows, g.d, g.gate_rows, g.kind, g.scale, g.eps);
+    out = ResidualNorm::apply(h, y, given(gate), given(w[0]), given(w[1]), given(w[2]), given(w[3]), g.rows, g.d, g.gate_rows, g.kind, g.scale, g.eps, g.expanded);
   } else {
     Tensor stats;
-    out = norm_forward(h, y, gate, w, g, false, stats);
+    out = norm_forward(h, y, whole_gate(gate, h, g.expanded), w, g, false, stats);
   }
   return {out[0], out[1]};
 }
 
 void bind(const std::vector<uintptr_t>& at) {
-  if (at.size() != 6) throw py::value_error("six entries are wanted");
+  if (at.size() != 8) throw py::value_error("eight entries are wanted");
   entries = {(decltype(entries.battn_fwd))at[0],   (decltype(entries.battn_bwd))at[1],   (decltype(entries.battn_ws))at[2],
-             (decltype(entries.resnorm_fwd))at[3], (decltype(entries.resnorm_bwd))at[4], (decltype(entries.resnorm_ws))at[5]};
+             (decltype(entries.resnorm_fwd))at[3], (decltype(entries.resnorm_bwd))at[4], (decltype(entries.resnorm_ws))at[5],
+             (decltype(entries.gate_sum))at[6],    (decltype(entries.gate_sum_ws))at[7]};
 }
 
 }  // namespace

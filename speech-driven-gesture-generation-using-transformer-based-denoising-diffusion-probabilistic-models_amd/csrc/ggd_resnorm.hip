@@ -40,6 +40,7 @@ struct RnBwd {
   int64_t per, groups; // per > 0: a block has `per` whole gate rows of the `groups` there are instead, and writes their sums itself
   int64_t group_rows;  // rows of a gate row (all rows without a gate, and where each row has its own)
   bool by_row;         // each row has its own gate row
+  bool gate32;         // ... and leaves its gradient in f32, for ggd_tr_gate_sum
 };
 
 // the thread's elements of a row: vector i covers columns (i TPR + t) V .. + V - 1
@@ -275,7 +276,8 @@ __global__ void __launch_bounds__(256) resnorm_bwd_kernel(RnBwd a) {
       if (a.by_row) {
 #pragma unroll
         for (int e = 0; e < E; ++e) du[e] = dt[e] * yn[e];
-        rn_store<T, V, NV, TPR>((T*)a.dgate + row * d, du, d, t);
+        if (a.gate32) rn_store<float, V, NV, TPR>((float*)a.dgate + row * d, du, d, t);
+        else rn_store<T, V, NV, TPR>((T*)a.dgate + row * d, du, d, t);
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) sgt[e] = fmaf(dt[e], yn[e], sgt[e]);
@@ -363,6 +365,88 @@ __global__ void __launch_bounds__(1024) resnorm_sum_kernel(RnSum a) {
   }
 }
 
+// Sums of an f32 array over some of its axes, those that a gate was broadcast along.  Neighbouring axes of one kind count as
+// one; where the last is kept a lane has an output, else a wave has, so that neighbouring lanes read neighbouring elements
+// either way.  Long sums are divided among blocks, whose parts gate_join_kernel adds.  Every sum has one order.  Bound
+// by reading the array once.
+constexpr int GS_AXES = 8;   // of each kind
+struct GateSum {
+  int kept, summed;                                   // axes, the last one first
+  int64_t kept_size[GS_AXES], kept_step[GS_AXES], summed_size[GS_AXES], summed_step[GS_AXES];
+  int64_t outs, terms, parts, blocks;                 // blocks: of 64 or 4 outputs
+  bool lanes;                                         // a lane an output
+};
+__device__ __forceinline__ int64_t gs_at(int64_t i, int axes, const int64_t* size, const int64_t* step) {
+  int64_t at = 0;
+  for (int k = 0; k < axes - 1; ++k) {
+    at += i % size[k] * step[k];
+    i /= size[k];
+  }
+  return axes ? at + i * step[axes - 1] : 0;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) gate_sum_kernel(GateSum a, const float* __restrict__ src, float* __restrict__ part, T* __restrict__ out) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t each = (a.terms + a.parts - 1) / a.parts, first = blockIdx.y * each, end = min(first + each, a.terms);
+  for (int64_t block = blockIdx.x; block < a.blocks; block += gridDim.x) {
+    const int64_t o = block * (a.lanes ? 64 : 4) + (a.lanes ? lane : wave);
+    float s = 0.f;
+    if (o < a.outs) {
+      const float* p = src + gs_at(o, a.kept, a.kept_size, a.kept_step);
+#pragma unroll 4
+      for (int64_t r = first + (a.lanes ? wave : lane); r < end; r += a.lanes ? 4 : 64) s += p[gs_at(r, a.summed, a.summed_size, a.summed_step)];
+    }
+    if (a.lanes) {
+      __syncthreads();
+      red[wave][lane] = s;
+      __syncthreads();
+      s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    } else {
+      float v[1] = {s};
+      rn_sum<64, 1>(v, nullptr);
+      s = v[0];
+    }
+    if (o >= a.outs || (a.lanes ? wave : lane)) continue;
+    if (a.parts > 1) part[blockIdx.y * a.outs + o] = s;
+    else out[o] = from_f32<T>(s);
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) gate_join_kernel(int64_t outs, int64_t parts, const float* __restrict__ part, T* __restrict__ out) {
+  const int64_t o = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);   // a wave an output
+  float s[1] = {0.f};
+  if (o < outs)
+    for (int64_t p = threadIdx.x & 63; p < parts; p += 64) s[0] += part[p * outs + o];
+  rn_sum<64, 1>(s, nullptr);
+  if (o < outs && (threadIdx.x & 63) == 0) out[o] = from_f32<T>(s[0]);
+}
+
+// 0, -1 (argument) or -2 (unsupported); the axes of one kind beside each other taken together, and 1024 blocks (of whole waves 4096, as their outputs may be few)
+int gs_plan(int axes, const int64_t* sizes, const uint8_t* kept, GateSum& a) {
+  a = GateSum{};
+  if (axes < 0 || (axes && (!sizes || !kept))) return -1;
+  a.outs = a.terms = 1;
+  int64_t step = 1;
+  int last = -1;
+  for (int i = axes - 1; i >= 0; --i) {
+    if (sizes[i] < 1 || step > INT64_MAX / sizes[i]) return -1;
+    if (sizes[i] == 1) continue;
+    const int k = kept[i] != 0;
+    int& n = k ? a.kept : a.summed;
+    if (k != last && n++ == GS_AXES) return -2;
+    (k ? a.kept_size : a.summed_size)[n - 1] = k == last ? (k ? a.kept_size : a.summed_size)[n - 1] * sizes[i] : sizes[i];
+    if (k != last) (k ? a.kept_step : a.summed_step)[n - 1] = step;
+    if (last < 0) a.lanes = k;
+    last = k;
+    step *= sizes[i];
+    (k ? a.outs : a.terms) *= sizes[i];
+  }
+  a.blocks = a.lanes ? (a.outs + 63) / 64 : (a.outs + 3) / 4;
+  a.parts = std::max<int64_t>(1, std::min<int64_t>((a.lanes ? 1024 : 4096) / a.blocks, a.terms / (a.lanes ? 64 : 1024)));
+  return 0;
+}
+
 bool rn_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int rn_check(const RnFwd& a, int dtype, int kind) {
@@ -448,17 +532,20 @@ int ggd_tr_resnorm_bwd(int64_t rows, int d, int dtype, int kind, float scale, fl
                        const float* pre_b, const float* stats, const void* dh_out, const void* du, void* dh, void* dy,
                        void* dgate, float* d_post_g, float* d_post_b, float* d_pre_g, float* d_pre_b, void* ws,
                        int64_t ws_bytes, void* stream) {
+  const bool gate32 = kind & GGD_TR_GATE_F32;
+  kind &= ~GGD_TR_GATE_F32;
   RnBwd a{};
   a.f = RnFwd{rows, gate_rows, d, kind, scale, eps, h, y, gate, post_g, post_b, pre_g, pre_b, dh, dy, (float*)stats};
   a.dho = dh_out, a.du = du, a.dh = dh, a.dy = dy, a.dgate = dgate, a.part = (float*)ws;
   if (const int e = rn_check(a.f, dtype, kind)) return e;
-  if (rows == 0 || !stats || !dh_out || !du || !gate != !dgate || !d_pre_g || !pre_b != !d_pre_b || !post_g != !d_post_g ||
+  if (rows == 0 || (gate32 && (!gate || gate_rows != 1)) || !stats || !dh_out || !du || !gate != !dgate || !d_pre_g || !pre_b != !d_pre_b || !post_g != !d_post_g ||
       !post_b != !d_post_b)
     return -1;
   if (!ws || !rn_aligned(ws) || ws_bytes < ggd_tr_resnorm_ws(rows, d, gate_rows, gate != nullptr)) return -1;
   const RnSegments g = rn_segments(rows, d, gate_rows, gate);
   a.seg = g.seg, a.segs = g.segs, a.per = g.per, a.groups = g.groups, a.group_rows = g.group_rows;
   a.by_row = gate && gate_rows == 1;
+  a.gate32 = gate32;
   const bool vec = d % (dtype == GGD_TR_F32 ? 4 : 8) == 0 && rn_aligned(h) && rn_aligned(y) && rn_aligned(gate) && rn_aligned(post_g) &&
                    rn_aligned(post_b) && rn_aligned(pre_g) && rn_aligned(pre_b) && rn_aligned(dh_out) && rn_aligned(du) &&
                    rn_aligned(dh) && rn_aligned(dy) && rn_aligned(dgate);
@@ -482,6 +569,29 @@ int ggd_tr_resnorm_bwd(int64_t rows, int d, int dtype, int kind, float scale, fl
     }
   r.lists = r.gate0 + (gate && !a.by_row && !g.per ? g.groups : 0);
   hipLaunchKernelGGL(resnorm_sum_kernel, dim3((d + 63) / 64, (unsigned)std::min<int64_t>(r.lists, 65535)), dim3(1024), 0, s, r);
+  return hipGetLastError() == hipSuccess ? 0 : -3;
+}
+
+int64_t ggd_tr_gate_sum_ws(int axes, const int64_t* sizes, const uint8_t* kept) {
+  GateSum a;
+  return gs_plan(axes, sizes, kept, a) || a.parts == 1 ? 0 : a.parts * a.outs * (int64_t)sizeof(float);
+}
+
+int ggd_tr_gate_sum(int axes, const int64_t* sizes, const uint8_t* kept, const float* src, int dtype, void* out, void* ws, int64_t ws_bytes,
+                    void* stream) {
+  GateSum a;
+  if (const int e = gs_plan(axes, sizes, kept, a)) return e;
+  if (!src || !out || (dtype != GGD_TR_F32 && dtype != GGD_TR_BF16)) return -1;
+  if (a.parts > 1 && (!ws || ws_bytes < a.parts * a.outs * (int64_t)sizeof(float))) return -1;
+  const dim3 grid((unsigned)std::min(a.blocks, RN_MAX_GRID), (unsigned)a.parts), join((unsigned)((a.outs + 3) / 4));
+  const hipStream_t s = (hipStream_t)stream;
+  if (dtype == GGD_TR_F32) {
+    hipLaunchKernelGGL(gate_sum_kernel<float>, grid, dim3(256), 0, s, a, src, (float*)ws, (float*)out);
+    if (a.parts > 1) hipLaunchKernelGGL(gate_join_kernel<float>, join, dim3(256), 0, s, a.outs, a.parts, (const float*)ws, (float*)out);
+  } else {
+    hipLaunchKernelGGL(gate_sum_kernel<bf16_t>, grid, dim3(256), 0, s, a, src, (float*)ws, (bf16_t*)out);
+    if (a.parts > 1) hipLaunchKernelGGL(gate_join_kernel<bf16_t>, join, dim3(256), 0, s, a.outs, a.parts, (const float*)ws, (bf16_t*)out);
+  }
   return hipGetLastError() == hipSuccess ? 0 : -3;
 }
 

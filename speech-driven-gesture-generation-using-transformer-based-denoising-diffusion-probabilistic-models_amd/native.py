@@ -51,7 +51,7 @@ EXPORTS = [
     "ggd_tr_mse", "ggd_tr_sumsq", "ggd_tr_sumsq_blocks", "ggd_tr_adamw", "ggd_tr_scale", "ggd_tr_scale_clamp",
     "ggd_tr_conv_fwd", "ggd_tr_conv_dgrad", "ggd_tr_conv_wgrad", "ggd_tr_im2col", "ggd_tr_col2im", "ggd_tr_batchnorm_fwd", "ggd_tr_batchnorm_bwd", "ggd_tr_image_channel_sum",
     "ggd_tr_channel_scale", "ggd_tr_pixel_shuffle", "ggd_tr_head_flatten", "ggd_enc_frontend",
-    "ggd_tr_resnorm_fwd", "ggd_tr_resnorm_bwd", "ggd_tr_resnorm_ws",
+    "ggd_tr_resnorm_fwd", "ggd_tr_resnorm_bwd", "ggd_tr_resnorm_ws", "ggd_tr_gate_sum", "ggd_tr_gate_sum_ws",
     "ggd_tr_battn_fwd", "ggd_tr_battn_bwd", "ggd_tr_battn_ws",
 ]
 
@@ -252,6 +252,8 @@ def load():
         "ggd_tr_resnorm_fwd": (ctypes.c_int, [I64, I32, I32, I32, F, F, VP, VP, VP, I64] + [VP] * 8),
         "ggd_tr_resnorm_bwd": (ctypes.c_int, [I64, I32, I32, I32, F, F, VP, VP, VP, I64] + [VP] * 15 + [I64, VP]),
         "ggd_tr_resnorm_ws": (I64, [I64, I32, I64, I32]),
+        "ggd_tr_gate_sum": (ctypes.c_int, [I32, VP, VP, VP, I32, VP, VP, I64, VP]),
+        "ggd_tr_gate_sum_ws": (I64, [I32, VP, VP]),
         # (a BattnArgs by reference, or its bytes)
         "ggd_tr_battn_fwd": (ctypes.c_int, [VP, VP]),
         "ggd_tr_battn_bwd": (ctypes.c_int, [VP, VP]),
@@ -283,7 +285,7 @@ def load_blocks():
         module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_blocks", BINDING, loader=loader))
         loader.exec_module(module)
         module.bind([ctypes.cast(getattr(lib, "ggd_tr_" + n), ctypes.c_void_p).value
-                     for n in ("battn_fwd", "battn_bwd", "battn_ws", "resnorm_fwd", "resnorm_bwd", "resnorm_ws")])
+                     for n in ("battn_fwd", "battn_bwd", "battn_ws", "resnorm_fwd", "resnorm_bwd", "resnorm_ws", "gate_sum", "gate_sum_ws")])
         _blocks = module
     return _blocks
 

@@ -251,3 +251,27 @@ def test_partial_sums_of_many_gate_rows_stay_few(native):
                 blocks = lib.ggd_tr_resnorm_ws(groups * rows, d, rows, 1) / (5 * d * 4)
                 assert 0 < blocks <= 4096, (d, groups, rows, blocks)
         assert lib.ggd_tr_resnorm_ws(1 << 30, d, 1, 0) / (5 * d * 4) <= 1024
+
+
+def test_gate_sum_entry_refusals(native):
+    lib = native.load()
+    at = 1 << 20
+
+    def call(sizes, kept, src=at, dtype=1, out=at, ws=None, ws_bytes=0, axes=None):
+        n = len(sizes)
+        return lib.ggd_tr_gate_sum(n if axes is None else axes, (ctypes.c_int64 * n)(*sizes), (ctypes.c_uint8 * n)(*kept), src, dtype, out, ws, ws_bytes, None)
+
+    def need(sizes, kept):
+        n = len(sizes)
+        return lib.ggd_tr_gate_sum_ws(n, (ctypes.c_int64 * n)(*sizes), (ctypes.c_uint8 * n)(*kept))
+
+    for bad in (dict(src=None), dict(out=None), dict(dtype=2), dict(axes=-1)):
+        assert call((2, 3), (1, 0), **bad) == -1, bad
+    assert call((2, 0), (1, 0)) == -1 and call((2, -3), (1, 0)) == -1 and call((1 << 40, 1 << 40), (1, 0)) == -1
+    assert lib.ggd_tr_gate_sum(2, None, None, at, 1, at, None, 0, None) == -1
+    assert call((2,) * 18, (1, 0) * 9) == -2 and need((2,) * 18, (1, 0) * 9) == 0
+    # axes of one kind in a row, and those of size 1, count as one: long sums of few outputs are divided
+    long = ((1, 3, 50, 1, 400, 2), (1, 0, 0, 1, 0, 1))
+    parts = need(*long) // (2 * 4)
+    assert parts > 1 and call(*long) == -1 and call(*long, ws=at, ws_bytes=need(*long) - 1) == -1
+    assert need((1 << 31, 64), (1, 0)) == 0 and need((1 << 20, 5), (0, 1)) == 1024 * 5 * 4

@@ -853,3 +853,64 @@ def test_residual_norm_with_millions_of_gate_rows(pkg):
     steps = 2 * (n // 4096 + 1) + 4 + 2048 // 16 + 16
     for a, b, c in zip(whole[5:], one[5:], two[5:]):
         assert bool(((a - (b + c)).abs() <= 2 * steps * U * 2 * n * 8).all())
+
+
+# gates that share elements of other axes than whole trailing rows: one a frame, one a token or clip, one for all, a middle axis
+GATES = [((3, 40, 96), (1, 40, 96)), ((3, 40, 96), (40, 96)), ((6, 50, 256), (6, 50, 1)), ((2, 9, 1024), (2, 1, 1)), ((2, 300, 65), (1, 1, 1)),
+         ((2, 300, 65), (1,)), ((2, 5, 4, 48), (2, 1, 4, 48)), ((2, 5, 4, 48), (1, 5, 1, 48)), ((2, 3, 5, 4, 8), (1, 3, 1, 4, 1)), ((700, 24), (700, 1)),
+         ((1, 5000, 33), (1, 5000, 1)), ((900, 2, 40), (1, 2, 40)), ((7,), (1,))]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape,lead", GATES, ids=str)
+def test_gradients_of_gates_that_broadcast_otherwise(pkg, shape, lead, dtype):
+    """The gradient of an element is one sum in f32, rounded once."""
+    h, y, pre, post, _ = norm_inputs(dtype, (1, *shape) if len(shape) < 2 else shape, "none")
+    h, y = h.reshape(shape), y.reshape(shape)
+    g = th.Generator().manual_seed(4)
+    gate = (th.randn(lead, generator=g) * 0.3 + 0.5).to(h.dtype).cuda()
+    dh, du = (th.randn(shape, generator=g).to(h.dtype).cuda() for _ in range(2))
+    leaves = [t.detach().requires_grad_() for t in (h, y, gate, *pre, *post)]
+    out = pkg.residual_norm(leaves[0], leaves[1], leaves[3:5], post=leaves[5:7], gate=leaves[2], scale=0.7)
+    got = th.autograd.grad(out, leaves, (dh, du))
+    d = shape[-1]
+    flat = lambda t: t.reshape(-1, d)
+    want, err, dgate, sums = norm_formula(flat(h), flat(y), flat(gate.expand(shape)), pre, post, 0.7, "layer", 1e-5, flat(dh), flat(du))
+    for name, a, b, e in zip(("h'", "u", "dh", "dy"), (*out, *got[:2]), want, err):
+        close(flat(a), b, e, name)
+    of = h.numel() // gate.numel()
+    x, e = (t.reshape(shape).sum_to_size(gate.shape) for t in (dgate[0], dgate[1] + of * U * dgate[0].abs()))
+    close(got[2], x, e + HALF[dtype] * (x.abs() + e), "dgate")
+    for a, (x, e) in zip(got[3:], sums):
+        close(a, x, e)
+
+
+def test_gates_that_broadcast_otherwise_are_captured(pkg):
+    """Replays of a pass whose gates' gradients are sums over other axes, in turn with eager work."""
+    g = th.Generator().manual_seed(8)
+    rnd = lambda *s: th.randn(*s, generator=g).bfloat16().cuda()
+    h, y, dh, du = (rnd(16, 512, 256) for _ in range(4))
+    w = th.ones(256, device="cuda")
+    for lead in ((1, 512, 256), (16, 512, 1), (1, 1, 1)):
+        leaves = [t.clone().requires_grad_() for t in (h, y, rnd(*lead))]
+
+        def both():
+            out = pkg.residual_norm(leaves[0], leaves[1], (w, None), gate=leaves[2], kind="rms")
+            return [*(o.detach() for o in out), *th.autograd.grad(out, leaves, (dh, du))]
+
+        side = th.cuda.Stream()
+        side.wait_stream(th.cuda.current_stream())
+        with th.cuda.stream(side):
+            both()
+        th.cuda.current_stream().wait_stream(side)
+        th.cuda.synchronize()
+        graph = th.cuda.CUDAGraph()
+        with th.cuda.graph(graph):
+            out = both()
+        for step in range(5):
+            with th.no_grad():
+                leaves[1].copy_(rnd(16, 512, 256))
+            want = [t.clone() for t in both()]
+            graph.replay()
+            th.cuda.synchronize()
+            assert all(th.equal(a, b) for a, b in zip(out, want)), (lead, step)
