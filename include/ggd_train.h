@@ -187,7 +187,8 @@ typedef struct ggd_tr_battn_args {
   /* kept for the backward pass (both null where none follows): [n][heads][lq][2], and o in f32, [n][lq][heads dk]
    * (f32: may be o itself where its rows are contiguous) */
   float *stat, *o32;
-  /* backward: dout, dq like o32's rows, dk and dv [n][lk][kv_heads dk], contiguous; dtable (nullable) [n_buckets][heads] */
+  /* backward: dout, dq like o32's rows, dk and dv (both null: not formed) [n][lk][kv_heads dk], contiguous; dtable (nullable)
+   * [n_buckets][heads] */
   const void* dout;
   void *dq, *dk_out, *dv;
   float* dtable;

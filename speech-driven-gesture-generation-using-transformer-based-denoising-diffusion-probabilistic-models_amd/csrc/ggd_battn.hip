@@ -130,7 +130,7 @@ Space backward_space(const BtArgs& a) {
   s.table = a.dtable ? up((int64_t)a.n * a.heads * ((a.lq + BT_ROWS - 1) / BT_ROWS) * (ds + two) * a.n_buckets * 4) : 0;
   s.rest = a.dtable && two ? up(2 * ds * (int64_t)a.n * a.heads * a.lq * 4) : 0;
   const int64_t pq = ds > 1 ? (int64_t)ds * a.n * a.lq * a.heads * a.dk * 4 : 0;
-  const int64_t pk = ks > 1 ? 2 * (int64_t)ks * a.n * a.lk * a.kv_heads * a.dk * 4 : 0;
+  const int64_t pk = ks > 1 && a.dk_out ? 2 * (int64_t)ks * a.n * a.lk * a.kv_heads * a.dk * 4 : 0;
   s.part = up(std::max(pq, pk));
   return s;
 }
@@ -203,7 +203,7 @@ int ggd_tr_battn_bwd(const ggd_tr_battn_args* args, void* stream) {
   BtArgs a{};
   if (const int e = prepare(args, a, true)) return e;
   if (a.n == 0) return 0;
-  if (!a.q || !a.k || !a.v || !a.stat || !a.o32 || !a.dout || !a.dq || !a.dk_out || !a.dv || (a.dtable && !a.table)) return -1;
+  if (!a.q || !a.k || !a.v || !a.stat || !a.o32 || !a.dout || !a.dq || !a.dk_out != !a.dv || (a.dtable && !a.table)) return -1;
   const Space space = backward_space(a);
   if (!a.ws || !aligned(a.ws, 16) || a.ws_bytes < space.all() || !aligned(a.stat, 8) || !aligned(a.o32, a.dk % 4 ? 4 : 16)) return -1;
   char* at = (char*)a.ws + space.pack;
@@ -218,6 +218,7 @@ int ggd_tr_battn_bwd(const ggd_tr_battn_args* args, void* stream) {
   if (rows(a, true, s) != hipSuccess) return -3;
   a.splits = dqs;
   if (launch(a).dq(a, s) != hipSuccess) return -3;
+  if (!a.dk_out) return 0;
   a.splits = dkvs;
   return launch(a).dkv(a, s) == hipSuccess ? 0 : -3;
 }

@@ -191,8 +191,10 @@ struct Attention : torch::autograd::Function<Attention> {
     {
       const at::NoGradGuard no_grad;
       const Tensor &stat = saved[7], &o32 = saved[8];
-      for (int i = 0; i < 3; ++i) out[i] = at::empty(saved[i].sizes(), saved[i].options());
-      if (in.table.defined() && in.table.requires_grad()) out[3] = at::empty(in.table.sizes(), in.table.options());
+      // dq's kernel also forms delta; dk and dv have one of their own, which a frozen memory does not need
+      const bool memory = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+      for (int i = 0; i < (memory ? 3 : 1); ++i) out[i] = at::empty(saved[i].sizes(), saved[i].options());
+      if (in.table.defined() && ctx->needs_input_grad(3)) out[3] = at::empty(in.table.sizes(), in.table.options());
       if (!stat.defined()) {
         for (Tensor& t : out)
           if (t.defined()) t.zero_();
@@ -201,7 +203,7 @@ struct Attention : torch::autograd::Function<Attention> {
         const Tensor dout = grads[0].contiguous();
         ggd_tr_battn_args a = args_of(in);
         a.stat = at_of<float>(stat), a.o32 = at_of<float>(o32), a.dout = dout.data_ptr();
-        a.dq = out[0].data_ptr(), a.dk_out = out[1].data_ptr(), a.dv = out[2].data_ptr(), a.dtable = at_of<float>(out[3]);
+        a.dq = out[0].data_ptr(), a.dk_out = at_of(out[1]), a.dv = at_of(out[2]), a.dtable = at_of<float>(out[3]);
         a.ws_bytes = entries.battn_ws(&a, 1);
         const Tensor ws = workspace(a.ws_bytes, in.q);
         a.ws = at_of(ws);
@@ -311,7 +313,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     variable_list out(14);
     {
       const at::NoGradGuard no_grad;
-      const bool expanded = saved[8].defined();
+      const bool expanded = saved[8].defined(), sum = expanded && ctx->needs_input_grad(2);
       const Tensor &h = saved[0], &y = saved[1], &gate = expanded ? saved[8] : saved[2], &stats = saved[7];
       for (int i = 0; i < 7; ++i)
         if (saved[i].defined()) out[i] = at::empty(saved[i].sizes(), saved[i].options());
@@ -323,13 +325,14 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const Tensor dh_out = grads[0].contiguous(), du = grads[1].contiguous();
         const int64_t bytes = entries.resnorm_ws(rows, (int)d, gate_rows, gate.defined());
         const Tensor ws = workspace(bytes, h);
-        const Tensor dgate = expanded ? at::empty(h.sizes(), h.options().dtype(at::kFloat)) : out[2];
-        const int rc = entries.resnorm_bwd(rows, (int)d, dtype_of(h), (int)kind | (expanded ? GGD_TR_GATE_F32 : 0), scale, eps, at_of(h), at_of(y), at_of(gate), gate_rows, at_of<float>(saved[3]),
+        const Tensor dgate = expanded ? at::empty(h.sizes(), sum ? h.options().dtype(at::kFloat) : h.options()) : out[2];
+        const int rc = entries.resnorm_bwd(rows, (int)d, dtype_of(h), (int)kind | (sum ? GGD_TR_GATE_F32 : 0), scale, eps, at_of(h), at_of(y), at_of(gate), gate_rows, at_of<float>(saved[3]),
                                            at_of<float>(saved[4]), at_of<float>(saved[5]), at_of<float>(saved[6]), at_of<float>(stats), at_of(dh_out),
                                            at_of(du), at_of(out[0]), at_of(out[1]), at_of(dgate), at_of<float>(out[3]), at_of<float>(out[4]),
                                            at_of<float>(out[5]), at_of<float>(out[6]), at_of(ws), bytes, stream_of(h));
         TORCH_CHECK(rc == 0, "residual_norm backward failed (ggd_train status ", rc, ")");
-        if (expanded) sum_gate(dgate, saved[2], out[2]);
+        if (sum) sum_gate(dgate, saved[2], out[2]);
+        else if (expanded) out[2] = Tensor();
       }
     }
     return once(std::move(out), "residual_norm");

@@ -275,3 +275,13 @@ def test_gate_sum_entry_refusals(native):
     parts = need(*long) // (2 * 4)
     assert parts > 1 and call(*long) == -1 and call(*long, ws=at, ws_bytes=need(*long) - 1) == -1
     assert need((1 << 31, 64), (1, 0)) == 0 and need((1 << 20, 5), (0, 1)) == 1024 * 5 * 4
+
+
+def test_backward_without_the_memorys_gradients(native):
+    """dk and dv both null: a valid call, without the workspace of their parts.  (ws left out: nothing is launched.)"""
+    lib = native.load()
+    shape = dict(n=1, heads=2, kv_heads=2, lq=2000, lk=300, dk=64, ldq=128, bq=256000, ldk=128, bk=38400, ldv=128, bv=38400, ldo=128, bo=256000)
+    need = [lib.ggd_tr_battn_ws(ctypes.byref(_battn(native, **shape, **over)), 1) for over in ({}, dict(dk_out=None, dv=None))]
+    assert 0 < need[1] < need[0]
+    for over in (dict(dk_out=None), dict(dv=None), dict(dk_out=None, dv=None, dq=None), dict(dk_out=None, dv=None, ws_bytes=need[1] - 1)):
+        assert lib.ggd_tr_battn_bwd(ctypes.byref(_battn(native, **shape, **over)), None) == -1, over

@@ -914,3 +914,35 @@ def test_gates_that_broadcast_otherwise_are_captured(pkg):
             graph.replay()
             th.cuda.synchronize()
             assert all(th.equal(a, b) for a, b in zip(out, want)), (lead, step)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradients_that_are_not_asked_for(pkg, dtype):
+    """Any operand frozen: the others' gradients have the same bits, and a frozen memory's dk and dv are not formed."""
+    n, lq, lk, heads, kv_heads, dk = 2, 70, 1500, 4, 2, 64
+    ins, do, _ = attention_inputs(dtype, n, lq, lk, heads, kv_heads, dk, n_buckets=8)
+    buckets = pkg.RelativeBuckets(8, 16)
+    want = run_attention(pkg, ins, do, heads, kv_heads, buckets=buckets)[1:]
+    for wanted in ((0,), (1,), (2,), (3,), (0, 3), (1, 2), (0, 1), (2, 3)):
+        leaves = [x.detach().requires_grad_(i in wanted) for i, x in enumerate(ins)]
+        o = pkg.relative_attention(*leaves[:3], heads, buckets, leaves[3], kv_heads=kv_heads)
+        got = th.autograd.grad(o, [leaves[i] for i in wanted], do)
+        assert all(th.equal(a, want[i]) for a, i in zip(got, wanted)), wanted
+    # dk and dv of a long memory alone would be twice its keys
+    q, k = (th.randn(1, rows, 64, device="cuda").to(DTYPES[dtype]) for rows in (8, 1 << 16))
+    q.requires_grad_()
+    o = pkg.cross_attention(q, k, k, 1)
+    before = th.cuda.memory_allocated()
+    th.cuda.reset_peak_memory_stats()
+    th.autograd.grad(o, [q], th.ones_like(o))
+    assert th.cuda.max_memory_allocated() - before < k.numel() * k.element_size()
+    h, y, pre, post, _ = norm_inputs(dtype, (3, 20, 64), "none")
+    gate = ins[3][:1, :1].to(h.dtype).reshape(1, 1, 1).expand(3, 20, 1).contiguous()
+    every = [h, y, gate, *pre, *post]
+    call = lambda t: pkg.residual_norm(t[0], t[1], t[3:5], post=t[5:7], gate=t[2])[1]
+    leaves = [t.detach().requires_grad_() for t in every]
+    want = th.autograd.grad(call(leaves), leaves, h)
+    for at in range(7):
+        leaves = [t.detach().requires_grad_(i == at) for i, t in enumerate(every)]
+        (got,) = th.autograd.grad(call(leaves), [leaves[at]], h)
+        assert th.equal(got, want[at]), at
