@@ -13,6 +13,8 @@ gradients wants leaves of which no eager graph is alive (a loss kept from before
 A wrong shape, type or device raises ValueError before anything is launched.  The checks, the allocations and
 the autograd nodes are in csrc/ggd_blocks.cpp.
 """
+import operator
+
 import numpy as np
 import torch as th
 
@@ -24,6 +26,21 @@ MAX_BUCKETS, MAX_DISTANCE = 1024, 2047   # include/ggd_train.h
 def _tensor(what, name, t):
     if not isinstance(t, th.Tensor):
         raise ValueError(f"{what}: {name} has to be a tensor")
+
+
+def _whole(what, name, x):
+    """A whole number, of any type that is one (a float is not, whatever its value)."""
+    try:
+        return operator.index(x)
+    except TypeError:
+        raise ValueError(f"{what}: {name} {x!r} has to be a whole number") from None
+
+
+def _number(what, name, x):
+    try:
+        return float(x)
+    except (TypeError, ValueError, OverflowError):
+        raise ValueError(f"{what}: {name} {x!r} has to be a number") from None
 
 
 # ------------------------------------------------------------------------------------------
@@ -41,7 +58,7 @@ class RelativeBuckets:
     """
 
     def __init__(self, n_buckets=32, max_distance=128, both_sides=True, device="cuda"):
-        n_buckets, max_distance = int(n_buckets), int(max_distance)
+        n_buckets, max_distance = _whole("RelativeBuckets", "n_buckets", n_buckets), _whole("RelativeBuckets", "max_distance", max_distance)
         side = n_buckets // 2 if both_sides else n_buckets
         if not 1 <= n_buckets <= MAX_BUCKETS or (both_sides and n_buckets % 2) or side < 2:
             raise ValueError(f"RelativeBuckets: n_buckets {n_buckets}: up to {MAX_BUCKETS}, at least 2 a side, even with both sides")
@@ -79,9 +96,10 @@ def _attention(what, q, k, v, heads, kv_heads, scale, mask, q_mask, lut, table, 
     try:
         return native.load_blocks().attention(what, q, k, v, heads, kv_heads, scale, mask, q_mask, lut, table, offset)
     except TypeError:
-        for name, t in (("q", q), ("k", k), ("v", v)):
-            _tensor(what, name, t)
-        raise
+        for name, t in (("q", q), ("k", k), ("v", v), ("mask", mask), ("q_mask", q_mask)):
+            if t is not None or len(name) == 1:
+                _tensor(what, name, t)
+        raise ValueError(f"{what}: heads {heads!r} and kv_heads {kv_heads!r} have to be whole numbers, scale {scale!r} a number") from None
 
 
 def cross_attention(q, k, v, heads, kv_heads=None, scale=None, mask=None, q_mask=None):
@@ -116,7 +134,8 @@ def relative_attention(q, k, v, heads, buckets, table, offset=0, kv_heads=None, 
     if table.dtype != th.float32 or table.shape != (buckets.n_buckets, heads):
         raise ValueError(f"{what}: table has to be ({buckets.n_buckets}, {heads}) in float32")
     lut = buckets.on(table.device) if table.is_cuda else None
-    return _attention(what, q, k, v, heads, kv_heads, scale, mask, q_mask, lut, table, max(-(1 << 62), min(1 << 62, int(offset))))
+    return _attention(what, q, k, v, heads, kv_heads, scale, mask, q_mask, lut, table,
+                      max(-(1 << 62), min(1 << 62, _whole(what, "offset", offset))))
 
 
 # ------------------------------------------------------------------------------------------
@@ -142,11 +161,12 @@ def residual_norm(h, y, pre, post=None, gate=None, scale=1.0, kind="layer", eps=
         post_g, post_b = (None, None) if post is None else post
     except (TypeError, ValueError):
         raise ValueError(f"{what}: pre and post have to be (weight, bias)") from None
-    if kind not in _KINDS:
+    if not isinstance(kind, str) or kind not in _KINDS:
         raise ValueError(f"{what}: kind {kind!r}: layer or rms")
+    scale, eps = _number(what, "scale", scale), _number(what, "eps", eps)
     try:
-        return native.load_blocks().residual_norm(h, y, pre_g, pre_b, post_g, post_b, gate, float(scale), _KINDS[kind], float(eps))
+        return native.load_blocks().residual_norm(h, y, pre_g, pre_b, post_g, post_b, gate, scale, _KINDS[kind], eps)
     except TypeError:
-        _tensor(what, "h", h)
-        _tensor(what, "y", y)
-        raise
+        for name, t in (("h", h), ("y", y)):
+            _tensor(what, name, t)
+        raise ValueError(f"{what}: weights, biases and gate have to be tensors or None") from None

@@ -6,6 +6,7 @@ import math
 import os
 import subprocess
 
+import numpy as np
 import pytest
 import torch as th
 
@@ -285,3 +286,27 @@ def test_backward_without_the_memorys_gradients(native):
     assert 0 < need[1] < need[0]
     for over in (dict(dk_out=None), dict(dv=None), dict(dk_out=None, dv=None, dq=None), dict(dk_out=None, dv=None, ws_bytes=need[1] - 1)):
         assert lib.ggd_tr_battn_bwd(ctypes.byref(_battn(native, **shape, **over)), None) == -1, over
+
+
+def test_arguments_of_another_kind_are_refused(pkg):
+    """ValueError, as documented, whatever an argument is; and no number is cut to a whole one."""
+    x, w = th.zeros(1, 2, 8), th.ones(8)
+    plan, table = pkg.RelativeBuckets(8, 16, device="cpu"), th.zeros(8, 2)
+    assert pkg.RelativeBuckets(np.int64(8), np.int32(16), device="cpu").buckets.equal(plan.buckets)
+    for call in (lambda: pkg.RelativeBuckets(8.0, 16, device="cpu"), lambda: pkg.RelativeBuckets(8, 16.9, device="cpu"),
+                 lambda: pkg.RelativeBuckets("8", 16, device="cpu"), lambda: pkg.RelativeBuckets(None, device="cpu")):
+        with pytest.raises(ValueError, match="whole number"):
+            call()
+    for over in (dict(heads="2"), dict(heads=2.5), dict(heads=None), dict(kv_heads=1.5), dict(scale="1"), dict(scale=x), dict(mask=[[True, True]]),
+                 dict(mask=1), dict(q_mask="all")):
+        args = dict(dict(heads=2), **over)
+        with pytest.raises(ValueError, match="has to be a tensor|whole numbers"):
+            pkg.cross_attention(x, x, x, **args)
+    for offset in (1.5, "1", None, x):
+        with pytest.raises(ValueError, match="offset"):
+            pkg.relative_attention(x, x, x, 2, plan, table, offset=offset)
+    for over, match in ((dict(pre=(1.0, None)), "tensors"), (dict(pre=("w", None)), "tensors"), (dict(gate=0.5), "tensors"), (dict(post=(w, 0)), "tensors"),
+                        (dict(kind=["layer"]), "layer or rms"), (dict(kind=None), "layer or rms"), (dict(scale="x"), "scale"), (dict(scale=None), "scale"),
+                        (dict(eps=w), "eps"), (dict(pre=w[0]), "weight, bias")):
+        with pytest.raises(ValueError, match=match):
+            pkg.residual_norm(x, x, **dict(dict(pre=(w, None)), **over))
