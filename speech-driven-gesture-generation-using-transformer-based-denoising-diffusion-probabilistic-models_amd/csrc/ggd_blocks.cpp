@@ -8,6 +8,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -246,6 +247,8 @@ Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tenso
   Inputs in{rows(q), rows(k), rows(v), Tensor(), mask_rows(what, "mask", mask, n, k.size(1)), mask_rows(what, "q_mask", q_mask, n, q.size(1)),
             or_none(buckets), heads, kv_heads, offset, scale};
   if (table) in.table = table->contiguous();
+  // (the plan's own memory, which no caller sees: let go while this stream works on it, it must not be handed on)
+  if (buckets) c10::hip::HIPCachingAllocator::recordStream(buckets->storage().data_ptr(), c10::hip::getCurrentHIPStream(q.device().index()));
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (table && table->requires_grad()));
   if (grad) check_capture(what, {q, k, v, or_none(table)});
   if (grad) return Attention::apply(in.q, in.k, in.v, given(in.table), given(in.mask), given(in.q_mask), given(in.buckets), heads, kv_heads, scale, offset);

@@ -946,3 +946,25 @@ def test_gradients_that_are_not_asked_for(pkg, dtype):
         leaves = [t.detach().requires_grad_(i == at) for i, t in enumerate(every)]
         (got,) = th.autograd.grad(call(leaves), [leaves[at]], h)
         assert th.equal(got, want[at]), at
+
+
+def test_a_plan_let_go_while_another_stream_uses_it(pkg):
+    """A plan made on one stream, used on a busy second one and dropped: its memory is not handed on before that use is over."""
+    ins, do, _ = attention_inputs("f32", 2, 40, 50, 2, 2, 32, n_buckets=8)
+    want = run_attention(pkg, ins, do, 2, 2, buckets=pkg.RelativeBuckets(8, 16))
+    busy = th.randn(4096, 4096, device="cuda")
+    side = th.cuda.Stream()
+    for _ in range(3):
+        plan = pkg.RelativeBuckets(8, 16)
+        size, at = plan.on("cuda").numel(), plan.on("cuda").data_ptr()
+        side.wait_stream(th.cuda.current_stream())
+        with th.cuda.stream(side):
+            for _ in range(20):
+                th.mm(busy, busy)
+            got = run_attention(pkg, ins, do, 2, 2, buckets=plan)
+        del plan
+        others = [th.full((size,), 7, dtype=th.int32, device="cuda") for _ in range(64)]   # on the first stream, at once
+        assert all(t.data_ptr() != at for t in others) or side.query()
+        th.cuda.synchronize()
+        assert all(th.equal(a, b) for a, b in zip(got, want))
+        del others
