@@ -413,6 +413,7 @@ void bind(const std::vector<uintptr_t>& at) {
 }  // namespace
 
 PYBIND11_MODULE(_blocks, m) {
+  m.attr("torch_version") = GGD_TORCH;
   m.def("bind", &bind);
   m.def("attention", &attention, py::call_guard<py::gil_scoped_release>());
   m.def("residual_norm", &residual_norm, py::call_guard<py::gil_scoped_release>());

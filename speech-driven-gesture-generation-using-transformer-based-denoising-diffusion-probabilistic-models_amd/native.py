@@ -17,6 +17,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 PRODUCT_LIB = os.path.join(PKG_DIR, "libggd.so")
 DIAG_LIB = os.path.join(PKG_DIR, "libggd_diag.so")
 BINDING = os.path.join(PKG_DIR, "_blocks.so")   # the decoder-block operators' calls (blocks.py), on torch's C++ side
+BINDING_TORCH = os.path.join(PKG_DIR, "build", "_blocks.torch")   # the torch it was built against
 LIB_PATH = DIAG_LIB if os.environ.get("GGD_DIAG") == "1" else PRODUCT_LIB
 # A/B experiments (scripts/ab.sh): another build of the same library, same ABI
 if os.environ.get("GGD_LIB"):
@@ -114,16 +115,28 @@ def is_stale():
     return _binding_is_stale()
 
 
+def _torch_version():
+    import torch
+    return str(torch.__version__)
+
+
 def _binding_is_stale():
-    return not os.path.exists(BINDING) or any(os.path.getmtime(p) > os.path.getmtime(BINDING)
-                                              for p in _deps(os.path.join(CSRC, BINDING_SOURCE)))
+    """Older than its sources, or built against another torch than the one that is here."""
+    if not os.path.exists(BINDING) or any(os.path.getmtime(p) > os.path.getmtime(BINDING) for p in _deps(os.path.join(CSRC, BINDING_SOURCE))):
+        return True
+    try:
+        with open(BINDING_TORCH) as f:
+            return f.read() != _torch_version()
+    except OSError:
+        return True
 
 
 def _binding_command():
     """g++ on the binding against torch's headers and libraries (which torch has loaded when it is)."""
     import sysconfig
     from torch.utils import cpp_extension
-    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"] +
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+             f'-DGGD_TORCH="{_torch_version()}"'] +
             ["-I" + d for d in cpp_extension.include_paths() + ["/opt/rocm/include", sysconfig.get_paths()["include"]]] +
             [os.path.join(CSRC, BINDING_SOURCE), "-o", BINDING + ".tmp"] + ["-L" + d for d in cpp_extension.library_paths()] +
             ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"])
@@ -165,6 +178,8 @@ def build(force=False, verbose=False):
         raise RuntimeError("hipcc failed")
     if binding:
         os.replace(BINDING + ".tmp", BINDING)
+        with open(BINDING_TORCH, "w") as f:
+            f.write(_torch_version())
     obj = lambda n: os.path.join(PKG_DIR, "build", n)
     product = [obj(s.replace(".hip", ".o")) for s in SOURCES]
     diag = [o for o in product if not o.endswith("ggd_api.o")] + [obj("ggd_api_diag.o"), obj("ggd_diag.o")]
@@ -284,6 +299,8 @@ def load_blocks():
         loader = importlib.machinery.ExtensionFileLoader("_blocks", BINDING)
         module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_blocks", BINDING, loader=loader))
         loader.exec_module(module)
+        if module.torch_version != _torch_version():
+            raise ImportError(f"{BINDING} was built against torch {module.torch_version}, here is {_torch_version()}; run __graft_entry__.build()")
         module.bind([ctypes.cast(getattr(lib, "ggd_tr_" + n), ctypes.c_void_p).value
                      for n in ("battn_fwd", "battn_bwd", "battn_ws", "resnorm_fwd", "resnorm_bwd", "resnorm_ws", "gate_sum", "gate_sum_ws")])
         _blocks = module

@@ -310,3 +310,18 @@ def test_arguments_of_another_kind_are_refused(pkg):
                         (dict(eps=w), "eps"), (dict(pre=w[0]), "weight, bias")):
         with pytest.raises(ValueError, match=match):
             pkg.residual_norm(x, x, **dict(dict(pre=(w, None)), **over))
+
+
+def test_the_binding_belongs_to_one_torch(native, monkeypatch):
+    """Another torch than the binding was built against: it counts as stale, and is not bound."""
+    if native.is_stale():
+        native.build()
+    assert not native._binding_is_stale() and native.load_blocks().torch_version == th.__version__
+    monkeypatch.setattr(th, "__version__", "0.1")
+    assert native._binding_is_stale() and native.is_stale()
+    monkeypatch.setattr(native, "_blocks", None)
+    with pytest.raises(ImportError, match="torch"):
+        native.load_blocks()
+    monkeypatch.undo()
+    monkeypatch.setattr(native, "BINDING_TORCH", native.BINDING_TORCH + ".none")
+    assert native._binding_is_stale()
