@@ -216,8 +216,12 @@ struct Attention : torch::autograd::Function<Attention> {
   }
 };
 
-// (n, L, W) with contiguous rows: the tensor where its rows are, whatever their strides, else a copy
-Tensor rows(const Tensor& t) { return t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+// (n, L, W) with contiguous rows: the tensor where its rows are, whatever their strides, else a copy (as of one whose values are negated
+// when they are read, by torch's operations alone)
+Tensor rows(const Tensor& x) {
+  const Tensor t = x.resolve_neg();
+  return t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
 
 Tensor mask_rows(const char* what, const char* name, const OptTensor& m, int64_t n, int64_t length) {
   if (!m) return Tensor();
@@ -246,7 +250,7 @@ Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tenso
   if (!((float)scale > 0.f && scale <= 1e30)) refuse(what, "scale ", scale, " has to be positive");
   Inputs in{rows(q), rows(k), rows(v), Tensor(), mask_rows(what, "mask", mask, n, k.size(1)), mask_rows(what, "q_mask", q_mask, n, q.size(1)),
             or_none(buckets), heads, kv_heads, offset, scale};
-  if (table) in.table = table->contiguous();
+  if (table) in.table = table->resolve_neg().contiguous();
   // (the plan's own memory, which no caller sees: let go while this stream works on it, it must not be handed on)
   if (buckets) c10::hip::HIPCachingAllocator::recordStream(buckets->storage().data_ptr(), c10::hip::getCurrentHIPStream(q.device().index()));
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (table && table->requires_grad()));
@@ -381,18 +385,19 @@ std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre
       beside(what, "a weight or bias", t, h);
       if (t.scalar_type() != at::kFloat || t.dim() != 1 || t.size(0) != d) refuse(what, "weights and biases have to be (", d, ",) in float32");
       grad = grad || t.requires_grad();
-      t = t.contiguous();
+      t = t.resolve_neg().contiguous();
     }
   if (!std::isfinite((float)scale) || !std::isfinite((float)eps) || !((float)eps > 0.f)) refuse(what, "scale ", scale, " has to be finite, eps ", eps, " positive");
   Shape g{h.numel() / d, d, 1, kind, scale, eps, false};
   Tensor gate = or_none(gate_in);
   if (gate.defined()) {
+    gate = gate.resolve_neg();
     g.gate_rows = gate_rows_of(what, gate, h);
     g.expanded = g.gate_rows == 0;
     if (g.expanded && h.dim() > 16) refuse(what, "a gate along other axes than whole trailing rows has to have at most 16");
     g.gate_rows = std::max<int64_t>(1, g.gate_rows);
   }
-  h = h.contiguous(), y = y.contiguous();
+  h = h.resolve_neg().contiguous(), y = y.resolve_neg().contiguous();
   variable_list out;
   if (grad && at::GradMode::is_enabled()) {
     out = ResidualNorm::apply(h, y, given(gate), given(w[0]), given(w[1]), given(w[2]), given(w[3]), g.rows, g.d, g.gate_rows, g.kind, g.scale, g.eps, g.expanded);

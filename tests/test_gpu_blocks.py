@@ -968,3 +968,16 @@ def test_a_plan_let_go_while_another_stream_uses_it(pkg):
         th.cuda.synchronize()
         assert all(th.equal(a, b) for a, b in zip(got, want))
         del others
+
+
+def test_values_negated_when_read(pkg):
+    """The imaginary part of a conjugate is a view whose values torch negates when it reads them."""
+    g = th.Generator().manual_seed(12)
+    neg = lambda *s: th.randn(*s, dtype=th.complex64, generator=g).cuda().conj().imag
+    q, k, v = neg(2, 3, 1), neg(2, 5, 1), neg(2, 5, 1)   # one head of one element: rows in place whatever the last stride
+    assert q.is_neg() and k.is_neg()
+    plain = [x.clone().resolve_neg() for x in (q, k, v)]
+    assert not plain[0].is_neg() and th.equal(pkg.cross_attention(q, k, v, 1), pkg.cross_attention(*plain, 1))
+    h, y, w, gate = neg(1, 1), neg(1, 1), neg(1), neg(1)
+    call = lambda f: pkg.residual_norm(f(h), f(y), (f(w), f(w)), post=(f(w), f(w)), gate=f(gate), kind="rms")
+    assert all(th.equal(a, b) for a, b in zip(call(lambda t: t), call(lambda t: t.clone().resolve_neg())))
