@@ -61,9 +61,11 @@ int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? GGD_TR_F3
 
 void on_gpu(const char* what, const Tensor& first) {
   if (!first.is_cuda()) refuse(what, "the inputs have to be on a GPU device (no CPU fallback)");
+  if (first.layout() != at::kStrided) refuse(what, "the inputs have to be dense tensors");
 }
 void beside(const char* what, const char* name, const OptTensor& t, const Tensor& first) {
   if (t && t->device() != first.device()) refuse(what, name, " has to be on ", first.device().str());
+  if (t && t->layout() != at::kStrided) refuse(what, name, " has to be a dense tensor");
 }
 
 template <typename T = void>

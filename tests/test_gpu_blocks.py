@@ -981,3 +981,15 @@ def test_values_negated_when_read(pkg):
     h, y, w, gate = neg(1, 1), neg(1, 1), neg(1), neg(1)
     call = lambda f: pkg.residual_norm(f(h), f(y), (f(w), f(w)), post=(f(w), f(w)), gate=f(gate), kind="rms")
     assert all(th.equal(a, b) for a, b in zip(call(lambda t: t), call(lambda t: t.clone().resolve_neg())))
+
+
+def test_sparse_tensors_are_refused(pkg):
+    x, w = th.ones(2, 3, 16, device="cuda"), th.ones(16, device="cuda")
+    keep = th.ones(2, 3, dtype=th.bool, device="cuda")
+    buckets, table = pkg.RelativeBuckets(8, 16), th.ones(8, 2, device="cuda")
+    for call in (lambda: pkg.cross_attention(x.to_sparse(), x, x, 2), lambda: pkg.cross_attention(x, x, x.to_sparse(), 2),
+                 lambda: pkg.cross_attention(x, x, x, 2, mask=keep.to_sparse()), lambda: pkg.relative_attention(x, x, x, 2, buckets, table.to_sparse()),
+                 lambda: pkg.residual_norm(x.to_sparse(), x, (w, w)), lambda: pkg.residual_norm(x, x.to_sparse(), (w, w)),
+                 lambda: pkg.residual_norm(x, x, (w.to_sparse(), w)), lambda: pkg.residual_norm(x, x, (w, w), gate=w.to_sparse())):
+        with pytest.raises(ValueError, match="dense"):
+            call()
