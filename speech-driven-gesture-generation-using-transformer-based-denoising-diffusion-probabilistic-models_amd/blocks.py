@@ -55,6 +55,9 @@ class RelativeBuckets:
     distances below s / 2 one bucket each; bucket s / 2 + k starts where
     |d| >= (s / 2) (max_distance / (s / 2)) ^ (k / (s - s / 2)) over the reals (compared in whole numbers,
     so that no logarithm rounds at a border), and distances from max_distance on share the last.
+
+    Neither form forbids the keys ahead by itself.  A causal model takes both sides with twice its buckets and a table whose second
+    half is -inf: relative_attention(..., torch.cat([table, table.new_full(table.shape, -math.inf)])).
     """
 
     def __init__(self, n_buckets=32, max_distance=128, both_sides=True, device="cuda"):
@@ -113,6 +116,10 @@ def cross_attention(q, k, v, heads, kv_heads=None, scale=None, mask=None, q_mask
     others is not read, their gradients are zero, and so is a row that may attend nothing (or that is
     not there).  Returns (n, Lq, heads dk).  Lengths from 0 on: few queries over a long memory -- a
     stream's newest frame -- divide the memory among the chip.
+    Sums, softmax and statistics are held in f32.  In bfloat16 the weights are rounded once for their product with v (and
+    with the gradients) in calls of more than 2^22 scores over more than 64 states, where results are off by that rounding
+    and their own; smaller calls, and few queries, carry them to 16 bits, so that the same clip may differ in its last bit alone and
+    in a batch.
     (Limits, past which there is a ValueError: 2^28 rows and states; clips x heads x (rows / 32, rounded up) up to 2^22; with
     gradients clips x kv_heads x (states / 128, rounded up) up to 2^22; rows of heads x dk below 32.5 MiB.)
     """

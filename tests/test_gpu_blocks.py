@@ -993,3 +993,23 @@ def test_sparse_tensors_are_refused(pkg):
                  lambda: pkg.residual_norm(x, x, (w.to_sparse(), w)), lambda: pkg.residual_norm(x, x, (w, w), gate=w.to_sparse())):
         with pytest.raises(ValueError, match="dense"):
             call()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lq,lk,offset", [(70, 70, 0), (300, 300, 0), (1, 90, 89), (5, 200, 195)])
+def test_a_causal_table(pkg, lq, lk, offset, dtype):
+    """Twice the buckets, the second half's entries -inf: each query attends the keys at and behind it, with the biases of a one-sided
+    plan, and the gradients of the learned half are those of the formula."""
+    n, heads, kv_heads, dk, s = 2, 4, 2, 32, 12
+    both, one = pkg.RelativeBuckets(2 * s, 40), pkg.RelativeBuckets(s, 40, both_sides=False)
+    assert th.equal(both.buckets[:41], one.buckets[:41])
+    ins, do, _ = attention_inputs(dtype, n, lq, lk, heads, kv_heads, dk, n_buckets=s)
+    table = th.cat([ins[3], th.full_like(ins[3], -math.inf)])
+    got = check_attention(pkg, [*ins[:3], table], do, heads, kv_heads, buckets=both, offset=offset)
+    assert not got[4][s:].any()
+    # keys ahead reach nothing, whatever they hold
+    if lq == 70:
+        late = [x.clone() for x in ins[:3]]
+        late[1][:, 40:], late[2][:, 40:] = 3., -5.
+        again = run_attention(pkg, [*late, table], do, heads, kv_heads, buckets=both, offset=offset)
+        assert th.equal(again[0][:, :40], got[0][:, :40])

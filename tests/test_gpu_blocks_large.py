@@ -30,6 +30,16 @@ def test_bf16_products_rounded_once(pkg, shape, relative):
     check_attention(pkg, ins, do, heads, kv_heads, mask=mask, q_mask=q_mask, buckets=buckets)
 
 
+def test_a_causal_table_in_a_large_call(pkg):
+    """The second half of both sides' buckets forbidden: most blocks of keys ahead have no place that is allowed."""
+    n, lq, lk, heads, kv_heads, dk = 2, 777, 777, 8, 2, 64
+    buckets = pkg.RelativeBuckets(24, 100)
+    ins, do, g = attention_inputs("bf16", n, lq, lk, heads, kv_heads, dk, n_buckets=12)
+    table = th.cat([ins[3], th.full_like(ins[3], -math.inf)])
+    got = check_attention(pkg, [*ins[:3], table], do, heads, kv_heads, mask=make_mask("ragged", n, lk, g), buckets=buckets)
+    assert not got[4][12:].any()
+
+
 @pytest.mark.parametrize("masked", [False, True])
 @pytest.mark.parametrize("n,heads,kv_heads,dk", [(8, 8, 8, 64), (8, 8, 2, 128), (16, 4, 1, 32)])
 def test_table_gradient_without_the_weights_rounding(pkg, n, heads, kv_heads, dk, masked):
