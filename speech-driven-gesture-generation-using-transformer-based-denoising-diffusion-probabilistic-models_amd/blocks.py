@@ -85,6 +85,10 @@ class RelativeBuckets:
         if th.device(device).type != "cpu":
             self.on(th.device(device))
 
+    def __getstate__(self):
+        """Without the copies on devices: those of the process that loads it are its own."""
+        return dict(self.__dict__, _on={})
+
     def on(self, device):
         """The buckets on a device, copied there once."""
         device = th.device(device)

@@ -238,6 +238,7 @@ Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tenso
   check_tangents(what, {q, k, v, or_none(table)});
   on_gpu(what, q);
   beside(what, "k", k, q), beside(what, "v", v, q), beside(what, "mask", mask, q), beside(what, "q_mask", q_mask, q), beside(what, "table", table, q);
+  beside(what, "the plan", buckets, q);
   const int64_t kv_heads = kv.value_or(heads);
   if (heads < 1 || kv_heads < 1 || heads % kv_heads) refuse(what, heads, " heads over ", kv_heads, " kv heads");
   if (q.dim() != 3 || k.dim() != 3 || v.dim() != 3) refuse(what, "q, k and v have to be (n, L, heads dk)");

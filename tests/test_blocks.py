@@ -1,9 +1,11 @@
 """CPU tests of the decoder-block operators (…_amd/blocks.py): the buckets' plan, the C structure's layout, and every
 refusal, in Python and at the C entries, none of which launches anything."""
+import copy
 import ctypes
 import importlib
 import math
 import os
+import pickle
 import subprocess
 
 import numpy as np
@@ -325,3 +327,12 @@ def test_the_binding_belongs_to_one_torch(native, monkeypatch):
     monkeypatch.undo()
     monkeypatch.setattr(native, "BINDING_TORCH", native.BINDING_TORCH + ".none")
     assert native._binding_is_stale()
+
+
+def test_a_plan_is_copied_without_its_devices(pkg):
+    """A loaded or copied plan makes its own copies on devices: those of another process, moved elsewhere on loading, would be read where
+    they are not."""
+    plan = pkg.RelativeBuckets(8, 16, device="cpu")
+    plan._on[th.device("cuda", 0)] = plan.on("cpu")   # what torch.load(..., map_location="cpu") made of a copy on a GPU
+    for other in (pickle.loads(pickle.dumps(plan)), copy.deepcopy(plan)):
+        assert other._on == {} and other.buckets.equal(plan.buckets) and (other.n_buckets, other.max_distance, other.both_sides) == (8, 16, True)

@@ -1013,3 +1013,15 @@ def test_a_causal_table(pkg, lq, lk, offset, dtype):
         late[1][:, 40:], late[2][:, 40:] = 3., -5.
         again = run_attention(pkg, [*late, table], do, heads, kv_heads, buckets=both, offset=offset)
         assert th.equal(again[0][:, :40], got[0][:, :40])
+
+
+def test_a_saved_plan_loaded_elsewhere(pkg, tmp_path):
+    ins, do, _ = attention_inputs("f32", 1, 40, 50, 2, 2, 32, n_buckets=8)
+    plan = pkg.RelativeBuckets(8, 16)
+    want = run_attention(pkg, ins, do, 2, 2, buckets=plan)
+    th.save(plan, tmp_path / "plan.pt")
+    loaded = th.load(tmp_path / "plan.pt", map_location="cpu", weights_only=False)
+    assert all(th.equal(a, b) for a, b in zip(run_attention(pkg, ins, do, 2, 2, buckets=loaded), want))
+    plan._on[th.device("cuda", 0)] = plan.buckets   # on the host: refused
+    with pytest.raises(ValueError, match="the plan"):
+        pkg.relative_attention(*ins[:3], 2, plan, ins[3])
