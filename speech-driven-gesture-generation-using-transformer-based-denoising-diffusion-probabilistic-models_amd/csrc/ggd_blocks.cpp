@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -114,6 +115,47 @@ void check_tangents(const char* what, at::ArrayRef<Tensor> inputs) {
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
 
+// (n, L, W) with contiguous rows: the tensor where its rows are, whatever their strides, else a copy (as of one whose values are negated
+// when they are read, by torch's operations alone)
+Tensor rows(const Tensor& x) {
+  const Tensor t = x.resolve_neg();
+  return t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
+
+// Saved tensors may come back through hooks that move them about.  The kernels read them by the types and sizes they had: a tensor of
+// another one, or on another device, is an error, and one laid out anew is read where it is now.
+// (The forms -- type and contiguity, then the sizes -- as bytes: a list's elements would be boxed one by one.)
+void save(AutogradContext* ctx, const variable_list& tensors) {
+  std::string forms;
+  auto add = [&](int64_t x) { forms.append((const char*)&x, sizeof(x)); };
+  for (const Tensor& t : tensors) {
+    add(t.defined() ? (int64_t)t.scalar_type() * 2 + t.is_contiguous() : -1);
+    if (t.defined()) forms.append((const char*)t.sizes().data(), t.dim() * sizeof(int64_t));
+  }
+  ctx->saved_data["forms"] = std::move(forms);
+  ctx->save_for_backward(tensors);
+}
+variable_list saved_by(AutogradContext* ctx, const char* what, const Tensor& like) {
+  variable_list tensors = ctx->get_saved_variables();
+  const std::string& forms = ctx->saved_data["forms"].toStringRef();
+  const char* at = forms.data();
+  for (Tensor& t : tensors) {
+    int64_t form;
+    std::memcpy(&form, at, sizeof(form));
+    at += sizeof(form);
+    bool same = t.defined() == (form >= 0);
+    if (same && t.defined()) {
+      const size_t bytes = t.dim() * sizeof(int64_t);
+      same = t.device() == like.device() && t.layout() == at::kStrided && (int64_t)t.scalar_type() == form / 2 &&
+             at + bytes <= forms.data() + forms.size() && std::memcmp(at, t.sizes().data(), bytes) == 0;
+      at += bytes;
+    }
+    TORCH_CHECK(same, what, " backward: a saved tensor came back on another device or of another type or shape");
+    if (t.defined() && !t.is_contiguous()) t = form & 1 ? t.contiguous() : rows(t);
+  }
+  return tensors;
+}
+
 // Gradients come once: where a graph of them is asked for, one that raises when it is used.
 variable_list once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -180,14 +222,14 @@ struct Attention : torch::autograd::Function<Attention> {
     Tensor stat, o32;
     const Inputs in{q, k, v, or_none(table), or_none(mask), or_none(q_mask), or_none(buckets), heads, kv_heads, offset, scale};
     Tensor o = attend(in, true, stat, o32);
-    ctx->save_for_backward({q, k, v, in.table, in.mask, in.q_mask, in.buckets, stat, o32});
+    save(ctx, {q, k, v, in.table, in.mask, in.q_mask, in.buckets, stat, o32});
     ctx->saved_data["heads"] = heads, ctx->saved_data["kv_heads"] = kv_heads, ctx->saved_data["scale"] = scale, ctx->saved_data["offset"] = offset;
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_traced("attention backward", grads);
     check_tangents("attention backward", grads);
-    const variable_list saved = ctx->get_saved_variables();
+    const variable_list saved = saved_by(ctx, "attention", grads[0]);
     const Inputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], ctx->saved_data["heads"].toInt(),
                     ctx->saved_data["kv_heads"].toInt(), ctx->saved_data["offset"].toInt(), ctx->saved_data["scale"].toDouble()};
     variable_list out(11);
@@ -217,13 +259,6 @@ struct Attention : torch::autograd::Function<Attention> {
     return once(std::move(out), "attention");
   }
 };
-
-// (n, L, W) with contiguous rows: the tensor where its rows are, whatever their strides, else a copy (as of one whose values are negated
-// when they are read, by torch's operations alone)
-Tensor rows(const Tensor& x) {
-  const Tensor t = x.resolve_neg();
-  return t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
-}
 
 Tensor mask_rows(const char* what, const char* name, const OptTensor& m, int64_t n, int64_t length) {
   if (!m) return Tensor();
@@ -308,7 +343,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const variable_list w{or_none(post_g), or_none(post_b), or_none(pre_g), or_none(pre_b)};
     const Tensor whole = whole_gate(or_none(gate), h, expanded);
     variable_list out = norm_forward(h, y, whole, w, {rows, d, gate_rows, kind, scale, eps, expanded}, true, stats);
-    ctx->save_for_backward({h, y, or_none(gate), w[0], w[1], w[2], w[3], stats, expanded ? whole : Tensor()});
+    save(ctx, {h, y, or_none(gate), w[0], w[1], w[2], w[3], stats, expanded ? whole : Tensor()});
     ctx->saved_data["rows"] = rows, ctx->saved_data["d"] = d, ctx->saved_data["gate_rows"] = gate_rows, ctx->saved_data["kind"] = kind;
     ctx->saved_data["scale"] = scale, ctx->saved_data["eps"] = eps;
     return out;
@@ -316,7 +351,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_traced("residual_norm backward", grads);
     check_tangents("residual_norm backward", grads);
-    const variable_list saved = ctx->get_saved_variables();
+    const variable_list saved = saved_by(ctx, "residual_norm", grads[0]);
     auto whole = [&](const char* name) { return ctx->saved_data[name].toInt(); };
     const int64_t rows = whole("rows"), d = whole("d"), gate_rows = whole("gate_rows"), kind = whole("kind");
     const float scale = (float)ctx->saved_data["scale"].toDouble(), eps = (float)ctx->saved_data["eps"].toDouble();

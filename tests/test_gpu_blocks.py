@@ -1025,3 +1025,36 @@ def test_a_saved_plan_loaded_elsewhere(pkg, tmp_path):
     plan._on[th.device("cuda", 0)] = plan.buckets   # on the host: refused
     with pytest.raises(ValueError, match="the plan"):
         pkg.relative_attention(*ins[:3], 2, plan, ins[3])
+
+
+def test_saved_tensors_through_hooks(pkg):
+    """Kept on the host in between, or laid out anew: the same gradients.  Come back on the host, of another type or shape: an error."""
+    hooks = th.autograd.graph
+    ins, do, g = attention_inputs("bf16", 2, 40, 50, 4, 2, 32, n_buckets=8)
+    buckets, mask = pkg.RelativeBuckets(8, 16), make_mask("ragged", 2, 50, g)
+    joint = th.cat([ins[1], ins[2]], -1)
+    h, y, pre, post, _ = norm_inputs("f32", (2, 5, 16), "none")
+    gate = th.rand(2, 5, 1, device="cuda")
+
+    def attend():
+        leaves = [x.detach().requires_grad_() for x in (ins[0], joint, ins[3])]
+        o = pkg.relative_attention(leaves[0], leaves[1][..., :64], leaves[1][..., 64:], 4, buckets, leaves[2], kv_heads=2, mask=mask)
+        return o, leaves, do
+
+    def norm():
+        leaves = [x.detach().requires_grad_() for x in (h, y, gate, *pre, *post)]
+        return pkg.residual_norm(leaves[0], leaves[1], leaves[3:5], post=leaves[5:], gate=leaves[2])[1], leaves, y
+
+    for make in (attend, norm):
+        want = th.autograd.grad(*make())
+        with hooks.save_on_cpu():
+            o = make()
+        assert all(th.equal(a, b) for a, b in zip(th.autograd.grad(*o), want))
+        with hooks.saved_tensors_hooks(lambda t: t, lambda t: t.transpose(0, -1).contiguous().transpose(0, -1)):
+            o = make()
+        assert all(th.equal(a, b) for a, b in zip(th.autograd.grad(*o), want))
+        for spoil in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t.flatten()[:-1], lambda t: t.unsqueeze(0), lambda t: t[..., :1]):
+            with hooks.saved_tensors_hooks(lambda t: t, spoil):
+                o = make()
+            with pytest.raises(RuntimeError, match="saved tensor"):
+                th.autograd.grad(*o)
