@@ -40,7 +40,6 @@ struct RnBwd {
   int64_t per, groups; // per > 0: a block has `per` whole gate rows of the `groups` there are instead, and writes their sums itself
   int64_t group_rows;  // rows of a gate row (all rows without a gate, and where each row has its own)
   bool by_row;         // each row has its own gate row
-  bool gate32;         // ... and leaves its gradient in f32, for ggd_tr_gate_sum
 };
 
 // the thread's elements of a row: vector i covers columns (i TPR + t) V .. + V - 1
@@ -198,11 +197,14 @@ __global__ void __launch_bounds__(256) resnorm_fwd_kernel(RnFwd a) {
 // weight gradients), the column sums stay in registers over the segment and leave as one row of partial
 // sums a block, which resnorm_sum_kernel adds in a fixed order.  Bound by HBM: bf16, 16 clips of 4096 rows of 1024, gate by
 // clip: 191 us for six tensors, 4.2 TB/s, and 11 us of column sums.
-template <typename T, int V, int NV, int TPR, bool SEVERAL>
+// (Forms of their own, so that none has another's registers: bf16 rows of 1024 take two waves a SIMD, just.)
+enum { RN_SEGMENT, RN_SEVERAL, RN_GATE32 };   // a segment; several gate rows; a segment that leaves each row's gate gradient in f32
+template <typename T, int V, int NV, int TPR, int FORM>
 __global__ void __launch_bounds__(256) resnorm_bwd_kernel(RnBwd a) {
   __shared__ float red[8];
   __shared__ float colred[TPR == 64 ? 3 * 64 * NV * V : 1];
   constexpr int E = NV * V, WAVES = 256 / TPR;
+  constexpr bool SEVERAL = FORM == RN_SEVERAL;
   const RnFwd& f = a.f;
   const int t = threadIdx.x & (TPR - 1), wave = TPR == 64 ? threadIdx.x >> 6 : 0, d = f.d;
   float ng[E], pg[E], sng[E], snb[E], spg[E], spb[E], sgt[E];
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(256) resnorm_bwd_kernel(RnBwd a) {
       if (a.by_row) {
 #pragma unroll
         for (int e = 0; e < E; ++e) du[e] = dt[e] * yn[e];
-        if (a.gate32) rn_store<float, V, NV, TPR>((float*)a.dgate + row * d, du, d, t);
+        if constexpr (FORM == RN_GATE32) rn_store<float, V, NV, TPR>((float*)a.dgate + row * d, du, d, t);
         else rn_store<T, V, NV, TPR>((T*)a.dgate + row * d, du, d, t);
       } else {
 #pragma unroll
@@ -545,18 +547,18 @@ int ggd_tr_resnorm_bwd(int64_t rows, int d, int dtype, int kind, float scale, fl
   const RnSegments g = rn_segments(rows, d, gate_rows, gate);
   a.seg = g.seg, a.segs = g.segs, a.per = g.per, a.groups = g.groups, a.group_rows = g.group_rows;
   a.by_row = gate && gate_rows == 1;
-  a.gate32 = gate32;
   const bool vec = d % (dtype == GGD_TR_F32 ? 4 : 8) == 0 && rn_aligned(h) && rn_aligned(y) && rn_aligned(gate) && rn_aligned(post_g) &&
                    rn_aligned(post_b) && rn_aligned(pre_g) && rn_aligned(pre_b) && rn_aligned(dh_out) && rn_aligned(du) &&
                    rn_aligned(dh) && rn_aligned(dy) && rn_aligned(dgate);
   hipStream_t s = (hipStream_t)stream;
 #define RN_GRID(TPR, K) hipLaunchKernelGGL(K, dim3((unsigned)g.blocks), dim3(256), 0, s, a)
   if (dtype == GGD_TR_F32) {
-    if (g.per) { RN_DISPATCH(resnorm_bwd_kernel, float, 4, vec, d, RN_GRID, , true) }
-    else { RN_DISPATCH(resnorm_bwd_kernel, float, 4, vec, d, RN_GRID, , false) }
+    if (g.per) { RN_DISPATCH(resnorm_bwd_kernel, float, 4, vec, d, RN_GRID, , RN_SEVERAL) }
+    else { RN_DISPATCH(resnorm_bwd_kernel, float, 4, vec, d, RN_GRID, , RN_SEGMENT) }   // (whose gate gradients are f32 anyway)
   } else {
-    if (g.per) { RN_DISPATCH(resnorm_bwd_kernel, bf16_t, 8, vec, d, RN_GRID, , true) }
-    else { RN_DISPATCH(resnorm_bwd_kernel, bf16_t, 8, vec, d, RN_GRID, , false) }
+    if (g.per) { RN_DISPATCH(resnorm_bwd_kernel, bf16_t, 8, vec, d, RN_GRID, , RN_SEVERAL) }
+    else if (gate32) { RN_DISPATCH(resnorm_bwd_kernel, bf16_t, 8, vec, d, RN_GRID, , RN_GATE32) }
+    else { RN_DISPATCH(resnorm_bwd_kernel, bf16_t, 8, vec, d, RN_GRID, , RN_SEGMENT) }
   }
 #undef RN_GRID
   RnSum r{};
