@@ -25,7 +25,7 @@ int prepare(const ggd_tr_battn_args* in, BtArgs& a, bool backward) {
     return -2;
   // rows that are packed lie their own width apart, and a tile of 64 of them is read by 32-bit byte offsets
   const int64_t head_bytes = (a.dk * (a.dtype == GGD_TR_F32 ? 4 : 2) + 15) / 16 * 16;
-  if (63 * a.heads * head_bytes + head_bytes > INT32_MAX) return -2;
+  if ((63 * (int64_t)a.heads + 1) * head_bytes > INT32_MAX) return -2;
   if (!a.table) a.distance = 0, a.n_buckets = 0;
   a.group = a.heads / a.kv_heads;
   if ((int64_t)a.group * a.lq > INT32_MAX - 64 || (int64_t)a.n * a.heads > 1 << 22 || (int64_t)a.heads * a.n_buckets > 1 << 25 ||

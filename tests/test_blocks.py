@@ -208,6 +208,8 @@ def test_rows_too_wide_for_their_offsets_are_unsupported(native, dtype, heads, d
     size = 4 if dtype == 0 else 2
     width = heads * ((dk * size + 15) // 16 * 16)
     assert 63 * width + 16 * ((dk * size + 15) // 16) > (1 << 31) - 1
+    most = _battn(native, n=0, heads=(1 << 31) - 1, kv_heads=1, dk=dk, dtype=dtype)   # (no clip: refused by the width alone)
+    assert lib.ggd_tr_battn_fwd(ctypes.byref(most), None) == -2
     for over, want in ((dict(heads=heads), -2), (dict(heads=heads // 2), -1)):
         args = _battn(native, n=1, kv_heads=1, lq=64, lk=64, dk=dk, dtype=dtype, ldq=8, bq=8, ldk=8, bk=8, ldv=8, bv=8, ws=None, ws_bytes=0, **over)
         assert lib.ggd_tr_battn_bwd(ctypes.byref(args), None) == want
