@@ -12,11 +12,14 @@
 // as the MFMA's M and the stationary row as the lane, so that a stationary row's scores lie in the
 // registers of two lanes (l and l ^ 32), the softmax needs one exchange between them, and the
 // probabilities are at once the B operand of the next product: its k slots may hold the streamed rows
-// in any order, as long as the A operand uses the same one (bt_acc).  No score goes through LDS.
+// in any order, as long as the A operand uses the same one (mma_cols).  Scores stay in registers; weights go through
+// LDS from one wave to another in the paired dk / dv kernel alone, and ds on their way into the table's sums by
+// diagonals.
 //   forward, dq:  stationary = queries (q, do), streamed = keys (k, v)
 //   dk, dv:       stationary = keys (k, v),     streamed = queries (q, do)
 // dq and dk / dv are two kernels that both form the scores (7 products instead of 5): the sums over
-// the streamed side then stay in registers, with neither atomics nor an order that varies.
+// the streamed side then stay in registers, with no order that varies (the table's sums by distance are LDS adds of
+// which no two meet on a word).
 #pragma once
 #include <hip/hip_runtime.h>
 

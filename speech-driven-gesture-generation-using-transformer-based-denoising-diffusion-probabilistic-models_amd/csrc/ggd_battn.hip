@@ -65,9 +65,9 @@ Packed packed_space(const BtArgs& a, bool backward) {
 
 // Few rows: the rows of a kv head's query heads fit one MFMA tile (32), or the call is small beside the keys it reads and the tiled
 // kernel's blocks of 128 rows would not fill the chip.  Blocks of 32 rows start sooner and divide finer: bf16, 8 heads of 64,
-// 128 rows over 16384 keys 31 us for the tiled kernel's 50, f32, 2 heads, 256 over 4096 26 for 35.  Past 2^24 scores they read each
-// key too often: bf16, 8 heads of 128, 1000 rows over 16000 271 us for 90, f32, 2 heads of 64, 4000 over 16000 408 for 286; and f32
-// heads past 64, of one wave a SIMD, past 2^22: 8 heads of 128, 256 over 4096 128 us for 70.
+// 128 rows over 16384 keys 32 us for the tiled kernel's 50, f32, 2 heads, 256 over 4096 25 for 35.  Past 2^24 scores they read each
+// key too often: bf16, 8 heads of 128, 1000 rows over 16000 297 us for 95, f32, 2 heads of 64, 4000 over 16000 442 for 327; and f32
+// heads past 64, of one wave a SIMD, past 2^22: 8 heads of 128, 256 over 4096 132 us for 73.
 bool few_rows(const BtArgs& a) {
   const int64_t rows = (int64_t)a.group * a.lq, blocks = (int64_t)a.n * a.heads * ((a.lq + BT_ROWS - 1) / BT_ROWS);
   const int64_t scores = a.dtype == GGD_TR_F32 && a.dk > 64 ? 1 << 22 : 1 << 24;
@@ -77,9 +77,8 @@ bool few_rows(const BtArgs& a) {
 // bf16 weights and ds, rounded once for their products, are off by up to 2^-8 each: a result's own rounding again, and over few
 // keys more in dq, where the roundings of o's weights do not average out in delta = do . o.  Where the call is small, or reads
 // its keys for few rows, a second product of what the rounding left costs little (few rows up to 32 are bound by their keys, more of them
-// up to 6 % of a training pass: 86 -> 91 us for 8 heads of 64, 256 rows over 8192): 33 -> 37 us of a training pass's
-// kernels at 2^21 scores (whose host side takes 65), 465 -> 493 at 256 clips x 8 heads, 500 over 64 keys; above it stays one, 100 -> 116 us
-// at 2^25 scores.
+// up to 7 % of a training pass's kernels: 86 -> 92 us for 8 heads of 64, 256 rows over 8192): 27 -> 30 us at 16 clips x 8 heads, 128 x 128
+// (whose host side takes 70), 485 -> 523 at 256 clips x 8 heads, 500 over 64 keys; above it stays one, 81 -> 98 us at 8 x 16 heads, 512 x 512.
 bool fine_weights(const BtArgs& a) {
   return a.dtype == GGD_TR_BF16 && (few_rows(a) || a.lk <= 64 || (int64_t)a.n * a.heads * a.lq <= (1 << 22) / a.lk);
 }

@@ -104,9 +104,10 @@ __device__ __forceinline__ void attend(Softmax<DK>& sm, const uint4* kimg, const
 // MFMA's N, and a tile of 64 keys in LDS (two: the next one arrives by LDS loads meanwhile) serves 4 of them.  Where blocks are
 // few the keys are divided too, and bt_join_kernel joins the parts.
 //   Bound by the VALU and the MFMA units, which two waves a SIMD overlap in part: exp, maximum and sum of a score are 4 VALU
-// operations a lane, and at dk = 64 take more time than its products (counters: VALU 70 %, MFMA 30 % of the cycles; no bank
-// conflict).  bf16, 8 clips x 16 heads, 4096 rows over 2048 keys, dk 128: 615 us, 670 TFLOP/s; 4 x 16 heads, 4096 over 4096, dk 64
-// with a bias: 409 us, 670.  f32, 4 x 8 heads, 600 over 1501, dk 64: 83 + 7 us in 3 parts, 67 TFLOP/s.
+// operations a lane, and at dk = 64 take more time than its products (counters, of the cycles a kernel runs: VALU 63 %, MFMA 31 %;
+// at dk 128 37 % and 30 %; no bank conflict).  bf16, 8 clips x 16 heads, 4096 rows over 2048 keys of which padding leaves about
+// three quarters, dk 128: 649 us, 635 TFLOP/s; 4 x 16 heads, 4096 over 4096, dk 64 with a bias: 415 us, 660.  f32, 4 x 8 heads,
+// 600 over 1501, padded like that, dk 64: 82 + 6 us in 3 parts, 67 TFLOP/s.  (These and the figures below: medians of one traced run.)
 // ---------------------------------------------------------------------------------------------
 template <typename T, int DK, bool BIAS>
 __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) bt_fwd_kernel(BtArgs a) {
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
 // fourth tile of 32 keys each, blocks a part of the keys (splits), and the parts are joined by their
 // maxima and sums.  Bound by reading the keys and values once: a wave has its next tile in flight
 // while it works on one, and needs no barrier for it.  bf16, 8 clips x 32 heads on 8 kv heads, one row over 32773 keys,
-// dk 128: 161 + 5 us, 5.0 TB/s; 32 clips x 8 heads over 1200, dk 64, with a bias: 20 + 4 us, 4.0 TB/s.
+// dk 128, three quarters left by padding: 165 + 5 us, 4.9 TB/s; 32 clips x 8 heads over 1200, dk 64, with a bias: 20 + 4 us, 3.9 TB/s.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ int64_t few_prow(const BtArgs& a, int64_t pair, int tiles, int tile) { return (pair * tiles + tile) * 32; }
 
@@ -364,8 +365,8 @@ __global__ void __launch_bounds__(256) bt_join_kernel(BtArgs a) {
 //   Table: ds go into a histogram over clamped distances, a copy a wave (diag_add); blocks past the table's distance
 // are summed in registers.
 //   Three products a score and one exp: bound by the MFMA and LDS reads that feed it (each 32 keys' image is read twice, by
-// rows and transposed).  The forward kernel's sizes: 716 us, 860 TFLOP/s at dk 128; 670 us, 615 at dk 64 with the table's
-// gradient; f32 118 + 7 us, 70.
+// rows and transposed).  The forward kernel's sizes: 743 us, 830 TFLOP/s at dk 128 (counters: MFMA 41 %, VALU 38 %); 675 us, 610 at
+// dk 64 with the table's gradient (28 %, 53 %); f32 118 + 7 us, 70.
 // ---------------------------------------------------------------------------------------------
 // the block's histogram copies and its lanes' sums past the distance -> a row of dtab.  first: the block's first query
 __device__ __forceinline__ void write_buckets(const BtArgs& a, float* hist, float past, float behind, int first, int64_t row) {
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1
 // f32 sum of many.  ds sum to zero over a row, so that what they do sum to is e_i, and each ds has p_ij e_i too
 // much: this kernel takes sum_i p_ij e_i off each distance's sum.  Only the places within the table's distance
 // are formed again (scores alone); the weights past it were summed on the way, and those behind are the remainder to 1.
-// 81 us of 4 x 16 heads, 4096 x 4096, distance 128, whose dq takes 670; 35 of 58 at 6 x 12 heads, 777 x 777, distance 200.
+// 80 us of 4 x 16 heads, 4096 x 4096, distance 128, whose dq takes 675; 36 beside 58 at 6 x 12 heads, 777 x 777, distance 200.
 template <typename T, int DK>
 __global__ void __launch_bounds__(256, 2) bt_table_rest_kernel(BtArgs a) {
   constexpr int KT = tile_rows<T, DK>(), IMG = KT * Img<T, DK>::UPR;
@@ -698,7 +699,7 @@ static __global__ void __launch_bounds__(64) bt_table_kernel(BtArgs a, int per, 
 // ---------------------------------------------------------------------------------------------
 // dk, dv: a block per 128 keys of a kv head; the queries of all its heads are streamed, head after head, so that
 // a shared head's gradient is one sum in registers.  Four products a score.  bf16 at dk 64 runs two waves a SIMD (4 x 16 heads,
-// 4096 x 4096: 725 us, 760 TFLOP/s); past 64 it has a kernel of its own below.  f32, 4 x 8 heads, 600 x 1501, dk 64: 168 us, 66 TFLOP/s.
+// 4096 x 4096: 717 us, 765 TFLOP/s; counters: MFMA 36 %, VALU 48 %); past 64 it has a kernel of its own below.  f32, 4 x 8 heads, 600 x 1501, dk 64: 167 us, 66 TFLOP/s.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int DK, bool BIAS>
 __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1) bt_dkv_kernel(BtArgs a) {
@@ -819,10 +820,11 @@ __global__ void __launch_bounds__(256, DK <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1)
 
 // ---------------------------------------------------------------------------------------------
 // dk, dv of bf16 heads past 64: two sums and two stationary rows are 400 registers, and one wave a SIMD overlaps nothing with its
-// products (1350 us at 8 clips x 4 kv heads of 4, 4096 x 2048, dk 128, padded; the MFMA 28 % busy).  So two waves share 32 keys: the first holds k and dv,
+// products (1350 us at 8 clips x 4 kv heads of 4, 4096 x 2048, dk 128, padded; 1206 with this kernel in the same run).  So two waves share 32 keys: the first holds k and dv,
 // forms the weights, p^T do and hands the weights on in f32 through LDS; the second, 32 queries behind, holds v and dk, forms
 // dp, ds and ds^T q.  Each has two of the four products, and a SIMD two waves.  A tile is in use for one and a half rounds: three
-// buffers.  1206 us, 680 TFLOP/s; what is left are the barrier after each 32 queries and the VALU work beside the products.
+// buffers.  Traced 1243 us, 660 TFLOP/s (counters: MFMA 31 %, VALU 27 %); what is left are the barrier after each 32 queries and the VALU
+// work beside the products.
 // ---------------------------------------------------------------------------------------------
 template <bool BIAS>
 __global__ void __launch_bounds__(512, 2) bt_dkv_pair_kernel(BtArgs a) {

@@ -135,8 +135,8 @@ __device__ __forceinline__ void rn_stats(const float (&x)[NV * V], int d, int t,
   rs = 1.0f / sqrtf(q[0] / d + eps);
 }
 
-// One row a wave (TPR 64, 4 rows a block) or a block (TPR 256).  Bound by HBM: bf16, 65536 rows of 1024: 112 us for four
-// tensors, 4.8 TB/s, the rate of a large copy.
+// One row a wave (TPR 64, 4 rows a block) or a block (TPR 256).  Bound by HBM: bf16, 65536 rows of 1024: 113 us for four
+// tensors, 4.7 TB/s, the rate of a large copy.
 template <typename T, int V, int NV, int TPR>
 __global__ void __launch_bounds__(256) resnorm_fwd_kernel(RnFwd a) {
   __shared__ float red[8];
