@@ -1058,3 +1058,54 @@ def test_saved_tensors_through_hooks(pkg):
                 o = make()
             with pytest.raises(RuntimeError, match="saved tensor"):
                 th.autograd.grad(*o)
+
+
+def test_threads_at_once(pkg):
+    """Each on a stream of its own, forward and backward: the bits of one alone."""
+    import threading
+    ins, do, _ = attention_inputs("bf16", 2, 60, 700, 4, 2, 64, n_buckets=8)
+    buckets = pkg.RelativeBuckets(8, 16)
+    h, y, pre, post, gate = norm_inputs("bf16", (4, 50, 256), "clip")
+
+    def both():
+        got = run_attention(pkg, ins, do, 4, 2, buckets=buckets)
+        leaves = [t.detach().requires_grad_() for t in (h, y, gate, *pre, *post)]
+        out = pkg.residual_norm(leaves[0], leaves[1], leaves[3:5], post=leaves[5:], gate=leaves[2])
+        return [*got, *out, *th.autograd.grad(out, leaves, (y, h))]
+
+    want, wrong = both(), []
+    th.cuda.synchronize()
+
+    def work():
+        stream = th.cuda.Stream()
+        with th.cuda.stream(stream):
+            for _ in range(20):
+                got = both()
+                stream.synchronize()
+                if not all(th.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_a_gate_whose_rows_are_not_in_order(pkg):
+    """A gate that is a transposed view, of the kinds that are read in place and that are expanded: gradients in its own order."""
+    h, y, pre, post, _ = norm_inputs("f32", (3, 20, 64), "none")
+    g = th.Generator().manual_seed(5)
+    for shape in ((1, 3, 64), (20, 3, 1), (64, 20, 1)):
+        base = th.randn(shape, generator=g).cuda()
+        views = {(1, 3, 64): lambda t: t.transpose(0, 1), (20, 3, 1): lambda t: t.transpose(0, 1), (64, 20, 1): lambda t: t.permute(2, 1, 0)}
+        view = views[shape]
+        grads = []
+        for leaf in (base.clone().requires_grad_(), view(base).contiguous().requires_grad_()):
+            gate = view(leaf) if leaf.shape == base.shape and not grads else leaf
+            out = pkg.residual_norm(h, y, pre, post=post, gate=gate)
+            (d,) = th.autograd.grad(out, [leaf], (y, h))
+            grads.append(view(d) if not grads else d)
+        assert th.equal(*grads), shape
+        check_norm(pkg, h, y, pre, post, view(base), 1.0, "layer") if shape[-1] == 64 else None

@@ -144,3 +144,20 @@ def test_many_heads_over_a_long_memory(pkg):
         err = (2 * 1200 * U + 2 * (dk + 8) * U * size.amax(-1, keepdim=True)) * want + U * want
         out = got.reshape(kv_heads, heads // kv_heads, dk)[h].double()
         assert bool(((out - want).abs() <= err).all()), (h, (out - want).abs().max().item(), err.max().item())
+
+
+@pytest.mark.parametrize("dk", [8, 128])
+def test_as_many_heads_as_there_may_be(pkg, dk):
+    """2^22 clips' heads of one row over one key: o is v, dv is do, and dq and dk nothing but the rounding of dk products twice."""
+    n, heads = 1 << 17, 32
+    q, k, v, do = (th.randn(n, 1, heads * dk, device="cuda", dtype=th.bfloat16) for _ in range(4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = pkg.cross_attention(*leaves, heads)
+    dq, dk_, dv = th.autograd.grad(o, leaves, do)
+    assert th.equal(o, v) and th.equal(dv, do)
+    for got, other in ((dq, k), (dk_, q)):
+        size = (do.float() * v.float()).abs().view(-1, dk).sum(-1).max() * other.float().abs().max()
+        assert got.float().abs().max() <= 2 * dk * U * size
+    more = th.zeros(n + 1, 1, heads * dk, device="cuda", dtype=th.bfloat16)
+    with pytest.raises(ValueError, match="unsupported shape"):
+        pkg.cross_attention(more, more, more, heads)
