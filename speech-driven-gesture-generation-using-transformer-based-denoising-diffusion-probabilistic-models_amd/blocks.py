@@ -36,13 +36,6 @@ def _whole(what, name, x):
         raise ValueError(f"{what}: {name} {x!r} has to be a whole number") from None
 
 
-def _number(what, name, x):
-    try:
-        return float(x)
-    except (TypeError, ValueError, OverflowError):
-        raise ValueError(f"{what}: {name} {x!r} has to be a number") from None
-
-
 # ------------------------------------------------------------------------------------------
 # attention
 # ------------------------------------------------------------------------------------------
@@ -174,9 +167,12 @@ def residual_norm(h, y, pre, post=None, gate=None, scale=1.0, kind="layer", eps=
         raise ValueError(f"{what}: pre and post have to be (weight, bias)") from None
     if not isinstance(kind, str) or kind not in _KINDS:
         raise ValueError(f"{what}: kind {kind!r}: layer or rms")
-    scale, eps = _number(what, "scale", scale), _number(what, "eps", eps)
     try:
-        return native.load_blocks().residual_norm(h, y, pre_g, pre_b, post_g, post_b, gate, scale, _KINDS[kind], eps)
+        numbers = float(scale), float(eps)
+    except (TypeError, ValueError, OverflowError):
+        raise ValueError(f"{what}: scale {scale!r} and eps {eps!r} have to be numbers") from None
+    try:
+        return native.load_blocks().residual_norm(h, y, pre_g, pre_b, post_g, post_b, gate, numbers[0], _KINDS[kind], numbers[1])
     except TypeError:
         for name, t in (("h", h), ("y", y)):
             _tensor(what, name, t)

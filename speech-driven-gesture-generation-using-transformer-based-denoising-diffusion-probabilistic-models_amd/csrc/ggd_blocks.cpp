@@ -97,36 +97,40 @@ void check_capture(const char* what, std::initializer_list<Tensor> inputs) {
   }
 }
 
-// A tracer sees the allocation of an output and not the kernels that fill it, and a tensor that only stands for another has no memory
-// to give them.
-void check_traced(const char* what, at::ArrayRef<Tensor> inputs) {
+// Calls that would be answered wrongly without an error.  A tracer sees the allocation of an output and not the kernels that fill it, and a
+// tensor that only stands for another has no memory to give them; and the kernels know no tangents, neither of inputs nor (in a backward
+// pass) of incoming gradients.
+const Tensor* there(const Tensor& t) { return t.defined() ? &t : nullptr; }
+const Tensor* there(const OptTensor& t) { return t && t->defined() ? &*t : nullptr; }
+template <typename... T>
+void check_plain(const char* what, const T&... inputs) {
   using Modes = c10::impl::TorchDispatchModeTLS;
   using Key = c10::impl::TorchDispatchModeKey;
-  bool traced = torch::jit::tracer::isTracing() || Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL) ||
-                c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
-  for (const Tensor& t : inputs) traced = traced || (t.defined() && t.unsafeGetTensorImpl()->is_python_dispatch());
+  bool traced = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+                (Modes::stack_len() && (Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL)));
+  const bool forward_mode = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  bool tangent = false;
+  auto look = [&](const Tensor* t) {
+    if (!t) return;
+    traced = traced || t->unsafeGetTensorImpl()->is_python_dispatch();
+    tangent = tangent || (forward_mode && t->_fw_grad(0).defined());
+  };
+  (look(there(inputs)), ...);
   TORCH_CHECK_NOT_IMPLEMENTED(!traced, what, " cannot be traced, nor called with fake tensors");
-}
-
-// The kernels know no tangents: one of an input's (or, in a backward pass, of an incoming gradient's) would be lost without an error.
-void check_tangents(const char* what, at::ArrayRef<Tensor> inputs) {
-  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-  for (const Tensor& t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+  TORCH_CHECK_NOT_IMPLEMENTED(!tangent, what, " has no forward-mode derivative");
 }
 
 // (n, L, W) with contiguous rows: the tensor where its rows are, whatever their strides, else a copy (as of one whose values are negated
 // when they are read, by torch's operations alone)
-Tensor rows(const Tensor& x) {
-  const Tensor t = x.resolve_neg();
-  return t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
-}
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor rows(const Tensor& t) { return t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? plain(t) : t.contiguous(); }
 
 // Saved tensors may come back through hooks that move them about.  The kernels read them by the types and sizes they had: a tensor of
 // another one, or on another device, is an error, and one laid out anew is read where it is now.
 // (The forms -- type and contiguity, then the sizes -- as bytes: a list's elements would be boxed one by one.)
 void save(AutogradContext* ctx, const variable_list& tensors) {
   std::string forms;
+  forms.reserve(512);
   auto add = [&](int64_t x) { forms.append((const char*)&x, sizeof(x)); };
   for (const Tensor& t : tensors) {
     add(t.defined() ? (int64_t)t.scalar_type() * 2 + t.is_contiguous() : -1);
@@ -227,8 +231,7 @@ struct Attention : torch::autograd::Function<Attention> {
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_traced("attention backward", grads);
-    check_tangents("attention backward", grads);
+    check_plain("attention backward", grads[0]);
     const variable_list saved = saved_by(ctx, "attention", grads[0]);
     const Inputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], saved[6], ctx->saved_data["heads"].toInt(),
                     ctx->saved_data["kv_heads"].toInt(), ctx->saved_data["offset"].toInt(), ctx->saved_data["scale"].toDouble()};
@@ -269,8 +272,7 @@ Tensor mask_rows(const char* what, const char* name, const OptTensor& m, int64_t
 
 Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tensor& v, int64_t heads, std::optional<int64_t> kv, std::optional<double> sc,
                  const OptTensor& mask, const OptTensor& q_mask, const OptTensor& buckets, const OptTensor& table, int64_t offset) {
-  check_traced(what, {q, k, v, or_none(mask), or_none(q_mask), or_none(table)});
-  check_tangents(what, {q, k, v, or_none(table)});
+  check_plain(what, q, k, v, mask, q_mask, table);
   on_gpu(what, q);
   beside(what, "k", k, q), beside(what, "v", v, q), beside(what, "mask", mask, q), beside(what, "q_mask", q_mask, q), beside(what, "table", table, q);
   beside(what, "the plan", buckets, q);
@@ -288,7 +290,7 @@ Tensor attention(const char* what, const Tensor& q, const Tensor& k, const Tenso
   if (!((float)scale > 0.f && scale <= 1e30)) refuse(what, "scale ", scale, " has to be positive");
   Inputs in{rows(q), rows(k), rows(v), Tensor(), mask_rows(what, "mask", mask, n, k.size(1)), mask_rows(what, "q_mask", q_mask, n, q.size(1)),
             or_none(buckets), heads, kv_heads, offset, scale};
-  if (table) in.table = table->resolve_neg().contiguous();
+  if (table) in.table = plain(*table).contiguous();
   // (the plan's own memory, which no caller sees: let go while this stream works on it, it must not be handed on)
   if (buckets) c10::hip::HIPCachingAllocator::recordStream(buckets->storage().data_ptr(), c10::hip::getCurrentHIPStream(q.device().index()));
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (table && table->requires_grad()));
@@ -349,8 +351,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    check_traced("residual_norm backward", grads);
-    check_tangents("residual_norm backward", grads);
+    check_plain("residual_norm backward", grads[0], grads[1]);
     const variable_list saved = saved_by(ctx, "residual_norm", grads[0]);
     auto whole = [&](const char* name) { return ctx->saved_data[name].toInt(); };
     const int64_t rows = whole("rows"), d = whole("d"), gate_rows = whole("gate_rows"), kind = whole("kind");
@@ -405,8 +406,7 @@ int64_t gate_rows_of(const char* what, Tensor& gate, const Tensor& h) {
 std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre_g, const OptTensor& pre_b, const OptTensor& post_g, const OptTensor& post_b,
                                         const OptTensor& gate_in, double scale, int64_t kind, double eps) {
   const char* what = "residual_norm";
-  check_traced(what, {h, y, or_none(gate_in), or_none(pre_g), or_none(pre_b), or_none(post_g), or_none(post_b)});
-  check_tangents(what, {h, y, or_none(gate_in), or_none(pre_g), or_none(pre_b), or_none(post_g), or_none(post_b)});
+  check_plain(what, h, y, gate_in, pre_g, pre_b, post_g, post_b);
   on_gpu(what, h);
   if (!pre_g || (!post_g && post_b)) refuse(what, "a norm needs a weight");
   beside(what, "y", y, h), beside(what, "gate", gate_in, h);
@@ -423,19 +423,19 @@ std::pair<Tensor, Tensor> residual_norm(Tensor h, Tensor y, const OptTensor& pre
       beside(what, "a weight or bias", t, h);
       if (t.scalar_type() != at::kFloat || t.dim() != 1 || t.size(0) != d) refuse(what, "weights and biases have to be (", d, ",) in float32");
       grad = grad || t.requires_grad();
-      t = t.resolve_neg().contiguous();
+      t = plain(t).contiguous();
     }
   if (!std::isfinite((float)scale) || !std::isfinite((float)eps) || !((float)eps > 0.f)) refuse(what, "scale ", scale, " has to be finite, eps ", eps, " positive");
   Shape g{h.numel() / d, d, 1, kind, scale, eps, false};
   Tensor gate = or_none(gate_in);
   if (gate.defined()) {
-    gate = gate.resolve_neg();
+    gate = plain(gate);
     g.gate_rows = gate_rows_of(what, gate, h);
     g.expanded = g.gate_rows == 0;
     if (g.expanded && h.dim() > 16) refuse(what, "a gate along other axes than whole trailing rows has to have at most 16");
     g.gate_rows = std::max<int64_t>(1, g.gate_rows);
   }
-  h = h.resolve_neg().contiguous(), y = y.resolve_neg().contiguous();
+  h = plain(h).contiguous(), y = plain(y).contiguous();
   variable_list out;
   if (grad && at::GradMode::is_enabled()) {
     out = ResidualNorm::apply(h, y, given(gate), given(w[0]), given(w[1]), given(w[2]), given(w[3]), g.rows, g.d, g.gate_rows, g.kind, g.scale, g.eps, g.expanded);
